@@ -343,6 +343,51 @@ int llm_lm_head_argmax_static(const int16_t* table, uint32_t vocab,
                               uint32_t ld, uint32_t row_count,
                               uint32_t* tokens, int64_t* scores, void* stream);
 
+/* No counterpart in the reference (its host takes the argmax alone).
+ * Next-token probabilities of rows [row0, row0 + rows) of `pair` through the
+ * LM head: probs, device memory [rows][vocab], receives Q0.32 values (raw
+ * 2^32 - 1 at most), temperatures[r] in [1/64, 64] dividing row r's scores.
+ * With s the exact int64 scores (20 fraction bits), c = floor(2^24 log2(e) /
+ * temperature + 1/2) and E[b][i] = floor(2^(30 - i / 2^b) + 1/2):
+ *   y_v = floor(min(max s - s_v, 2^31) c / 2^24),
+ *   w_v = floor(E[10][y / 2^10 mod 2^10] E[20][y mod 2^10] / 2^30) >> (y >> 20),
+ *   P_v = min(floor(2^32 w_v / sum w), 2^32 - 1)
+ * (quotients of y rounded down): e^((s_v - max s) / T) / sum to about 2^-20 of
+ * its value and 2^-32.  Work is enqueued on the context stream and not waited
+ * for.  The first call, and the first after a larger LM head was loaded,
+ * allocates (call it once before capturing a graph); the scores' memory is
+ * the context's, so graphs that hold such calls must not run beside one
+ * another or beside the context's own work. */
+int llm_lm_head_probs(llm_ctx_t* ctx, uint32_t pair, uint32_t row0, uint32_t rows,
+                      const double* temperatures, uint32_t* probs);
+
+/* No counterpart in the reference.  Verification of the drafted tokens of
+ * `requests` requests against these probabilities, and each request's next
+ * token, from random numbers of the caller's.  The requests' rows lie in
+ * `pair` from row0 on, one after the other: request j has draft_counts[j]
+ * (0 ..) drafted tokens and one row more, at most 8 rows in all; its row i is
+ * the hidden row (after the final norm) that its draft i is tested in, the
+ * last row the one after all its drafts.  drafts and accept_u hold one value
+ * per draft, sample_u and temperatures (see above) one per request; u are
+ * uniform 32-bit numbers.  draft_probs, device memory [drafts][vocab] Q0.32,
+ * are the distributions Q that the drafts were sampled from; NULL: the
+ * drafter had no choice (looked-up or greedy drafts), Q = 2^32 - 1 on the
+ * draft.  Draft x of a row is taken iff accept_u Q_x < 2^32 P_x; drafts after
+ * the first that is not taken are not considered.  The next token is drawn in
+ * that draft's row from max(P - Q, 0), or from P in the row after the drafts
+ * or where max(P - Q, 0) is 0 everywhere: the first token whose running sum
+ * passes floor(sample_u R / 2^32), R the whole sum.  So the tokens are
+ * distributed as if each had been sampled from P; with no drafts this is
+ * plain sampling.
+ * Host memory: accepted[requests], tokens[requests] (the drawn ones) and,
+ * unless NULL, probs[rows]: P of each draft, and at a request's last row P of
+ * its drawn token.  Waits for the result.  Allocates as llm_lm_head_probs. */
+int llm_lm_head_verify(llm_ctx_t* ctx, uint32_t pair, uint32_t row0, uint32_t requests,
+                       const uint32_t* draft_counts, const uint32_t* drafts,
+                       const uint32_t* accept_u, const uint32_t* sample_u,
+                       const double* temperatures, const uint32_t* draft_probs,
+                       uint32_t* accepted, uint32_t* tokens, uint32_t* probs);
+
 /* Report of llm_generate (the QWEN_8X64_E2E_PROFILE fields of the
  * reference's generate mode, host/host_qwen_8x64.cpp:9264-9336).  Forward
  * and LM-head times are stream-event times on the device (a forward from

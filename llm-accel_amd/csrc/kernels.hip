@@ -968,13 +968,17 @@ __global__ __launch_bounds__(64 * KS) void proj_mfma12_kernel(ProjArgs a, uint32
 // at most kLmStageSteps k-steps) and every step reads them from there, so
 // that the loads in the loop are the table's only (the four lanes of a
 // column group read the same 16 bytes: an LDS broadcast).
+// SC: the scores themselves are kept too, scores[r][v] of row stride lds (a
+// multiple of 16).
 constexpr uint32_t kLmStageSteps = 32;
-template <int RT, int L, bool XS = false>
+template <int RT, int L, bool XS = false, bool SC = false>
 __global__ __launch_bounds__(256) void lm_argmax_kernel(const int16_t* __restrict__ w,
                                                         uint32_t S, uint32_t n,
                                                         const int16_t* __restrict__ x,
                                                         uint32_t ldx, uint32_t rows,
-                                                        unsigned long long* keys) {
+                                                        unsigned long long* keys,
+                                                        int64_t* __restrict__ scores,
+                                                        uint32_t lds) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int i = lane >> 4, j = lane & 15;
     const uint32_t nblocks = (n + 3) / 4;
@@ -1035,6 +1039,7 @@ __global__ __launch_bounds__(256) void lm_argmax_kernel(const int16_t* __restric
             acc[r] = row16_sum(acc[r]);
             const unsigned long long k = argmax_key(acc[r], v);
             if (j == 15 && v < n && k > best[r]) best[r] = k;
+            if (SC && j == 15 && v < n && r < (int)rows) scores[(size_t)r * lds + v] = acc[r];
         }
     }
     __shared__ unsigned long long wbest[4][4][RT];
@@ -1068,12 +1073,14 @@ __global__ __launch_bounds__(256) void lm_argmax_kernel(const int16_t* __restric
 constexpr uint32_t kLmGroup = 16;
 // Activations of at most 60 KiB (44 with the shared groups' sums) in LDS.
 constexpr uint32_t kLmMfmaSteps = 30, kLmMfmaStepsShared = 22;
-template <bool KS>
+template <bool KS, bool SC = false>
 __global__ __launch_bounds__(256) void lm_argmax_mfma_kernel(const int16_t* __restrict__ w,
                                                              uint32_t S, uint32_t n,
                                                              const int16_t* __restrict__ x,
                                                              uint32_t ldx, uint32_t rows,
-                                                             unsigned long long* keys) {
+                                                             unsigned long long* keys,
+                                                             int64_t* __restrict__ scores,
+                                                             uint32_t lds) {
     extern __shared__ __attribute__((aligned(16))) int8_t lm_x[];  // [S][2][64][16]
     __shared__ int32_t xsum[8];
     __shared__ unsigned long long wbest[4][16];
@@ -1175,6 +1182,8 @@ __global__ __launch_bounds__(256) void lm_argmax_mfma_kernel(const int16_t* __re
             const uint32_t v = kLmGroup * gr + 4 * g + t;
             const unsigned long long k = argmax_key(score, v);
             if (v < n && k > best) best = k;
+            if (SC && j < rows && v < n && (!KS || wave == 0))
+                scores[(size_t)j * lds + v] = score;
         }
     }
     // the best of a row's lanes (g), then of the wavefronts
@@ -1192,10 +1201,11 @@ __global__ __launch_bounds__(256) void lm_argmax_mfma_kernel(const int16_t* __re
     }
 }
 
-template <int RT>
+template <int RT, bool SC>
 static hipError_t launch_lm_rt(const int16_t* w, uint32_t steps, uint32_t n,
                                const int16_t* x, uint32_t ldx, uint32_t rows, int L,
-                               unsigned long long* keys, hipStream_t st) {
+                               unsigned long long* keys, int64_t* scores, uint32_t lds,
+                               hipStream_t st) {
     const uint32_t nblocks = (n + 3) / 4;
     // Every workgroup ends with one atomicMax per row on the same line, and
     // every wavefront adds to the loads in flight.  One staged row streams the
@@ -1213,27 +1223,28 @@ static hipError_t launch_lm_rt(const int16_t* w, uint32_t steps, uint32_t n,
     if (staged) {
         constexpr bool XS = RT <= 2;
         switch (L) {
-        case 0: lm_argmax_kernel<RT, 0, XS><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys); break;
-        case 1: lm_argmax_kernel<RT, 1, XS><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys); break;
-        case 4: lm_argmax_kernel<RT, 4, XS><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys); break;
-        case 8: lm_argmax_kernel<RT, 8, XS><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys); break;
-        default: lm_argmax_kernel<RT, 16, XS><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys); break;
+        case 0: lm_argmax_kernel<RT, 0, XS, SC><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys, scores, lds); break;
+        case 1: lm_argmax_kernel<RT, 1, XS, SC><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys, scores, lds); break;
+        case 4: lm_argmax_kernel<RT, 4, XS, SC><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys, scores, lds); break;
+        case 8: lm_argmax_kernel<RT, 8, XS, SC><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys, scores, lds); break;
+        default: lm_argmax_kernel<RT, 16, XS, SC><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys, scores, lds); break;
         }
         return hipGetLastError();
     }
     switch (L) {
-    case 0: lm_argmax_kernel<RT, 0><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys); break;
-    case 1: lm_argmax_kernel<RT, 1><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys); break;
-    case 4: lm_argmax_kernel<RT, 4><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys); break;
-    case 8: lm_argmax_kernel<RT, 8><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys); break;
-    default: lm_argmax_kernel<RT, 16><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys); break;
+    case 0: lm_argmax_kernel<RT, 0, false, SC><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys, scores, lds); break;
+    case 1: lm_argmax_kernel<RT, 1, false, SC><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys, scores, lds); break;
+    case 4: lm_argmax_kernel<RT, 4, false, SC><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys, scores, lds); break;
+    case 8: lm_argmax_kernel<RT, 8, false, SC><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys, scores, lds); break;
+    default: lm_argmax_kernel<RT, 16, false, SC><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys, scores, lds); break;
     }
     return hipGetLastError();
 }
 
-hipError_t launch_lm_argmax(const int16_t* w, uint32_t steps, uint32_t n,
-                            const int16_t* x, uint32_t ldx, uint32_t rows, int L,
-                            unsigned long long* keys, hipStream_t st) {
+template <bool SC>
+static hipError_t launch_lm(const int16_t* w, uint32_t steps, uint32_t n, const int16_t* x,
+                            uint32_t ldx, uint32_t rows, int L, unsigned long long* keys,
+                            int64_t* scores, uint32_t lds, hipStream_t st) {
     // From three rows on the matrix cores (call times, dot2 -> matrix cores:
     // 151,936 x 2,048, 3 rows 236 -> 127-135 us, 8 415 -> 128-135; 151,936 x
     // 896 98 -> 57, 157 -> 57; 16,384 x 896 35 -> 22, 39 -> 22; 8,192 x 256
@@ -1247,17 +1258,31 @@ hipError_t launch_lm_argmax(const int16_t* w, uint32_t steps, uint32_t n,
     const uint32_t groups = (n + kLmGroup - 1) / kLmGroup;
     const bool shared = groups < 2048;
     if (rows >= 3 && steps <= (shared ? kLmMfmaStepsShared : kLmMfmaSteps)) {
-        const uint32_t lds = steps * 2048;
+        const uint32_t bytes = steps * 2048;  // of LDS
         if (shared)
-            lm_argmax_mfma_kernel<true><<<std::min(groups, 512u), 256, lds, st>>>(w, steps, n, x, ldx, rows, keys);
+            lm_argmax_mfma_kernel<true, SC><<<std::min(groups, 512u), 256, bytes, st>>>(
+                w, steps, n, x, ldx, rows, keys, scores, lds);
         else
-            lm_argmax_mfma_kernel<false><<<256, 256, lds, st>>>(w, steps, n, x, ldx, rows, keys);
+            lm_argmax_mfma_kernel<false, SC><<<256, 256, bytes, st>>>(w, steps, n, x, ldx, rows,
+                                                                      keys, scores, lds);
         return hipGetLastError();
     }
-    if (rows <= 1) return launch_lm_rt<1>(w, steps, n, x, ldx, rows, L, keys, st);
-    if (rows <= 2) return launch_lm_rt<2>(w, steps, n, x, ldx, rows, L, keys, st);
-    if (rows <= 4) return launch_lm_rt<4>(w, steps, n, x, ldx, rows, L, keys, st);
-    return launch_lm_rt<8>(w, steps, n, x, ldx, rows, L, keys, st);
+    if (rows <= 1) return launch_lm_rt<1, SC>(w, steps, n, x, ldx, rows, L, keys, scores, lds, st);
+    if (rows <= 2) return launch_lm_rt<2, SC>(w, steps, n, x, ldx, rows, L, keys, scores, lds, st);
+    if (rows <= 4) return launch_lm_rt<4, SC>(w, steps, n, x, ldx, rows, L, keys, scores, lds, st);
+    return launch_lm_rt<8, SC>(w, steps, n, x, ldx, rows, L, keys, scores, lds, st);
+}
+
+hipError_t launch_lm_argmax(const int16_t* w, uint32_t steps, uint32_t n,
+                            const int16_t* x, uint32_t ldx, uint32_t rows, int L,
+                            unsigned long long* keys, hipStream_t st) {
+    return launch_lm<false>(w, steps, n, x, ldx, rows, L, keys, nullptr, 0, st);
+}
+hipError_t launch_lm_scores(const int16_t* w, uint32_t steps, uint32_t n,
+                            const int16_t* x, uint32_t ldx, uint32_t rows, int L,
+                            unsigned long long* keys, int64_t* scores, uint32_t lds,
+                            hipStream_t st) {
+    return launch_lm<true>(w, steps, n, x, ldx, rows, L, keys, scores, lds, st);
 }
 
 // ---------------------------------------------------------------------

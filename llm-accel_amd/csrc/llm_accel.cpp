@@ -28,6 +28,7 @@
 #include "kernels.h"
 #include "ops.h"
 #include "prefill.h"
+#include "verify.h"
 
 namespace {
 
@@ -245,6 +246,20 @@ struct llm_ctx {
     Matrix lm;
     uint32_t lm_vocab = 0;
     unsigned long long* lm_keys = nullptr;
+    // Next-token probabilities and draft verification (verify.h), made by the
+    // first such call: every row's scores (replaced by a larger allocation for
+    // a larger vocabulary; the old one stays the context's, for captured
+    // graphs that hold it), the powers of two, the passes' sums, and the
+    // verification's words in pinned host memory.
+    struct Probs {
+        int64_t* scores = nullptr;
+        size_t lds = 0;
+        uint32_t* exp2 = nullptr;
+        int64_t* top = nullptr;
+        unsigned long long *part = nullptr, *left = nullptr;
+        uint32_t* count = nullptr;
+        uint32_t* host = nullptr;
+    } probs;
 
     // Request loop (llm_generate): pinned staging of the embedding rows of
     // one request (copied to the device asynchronously, one forward's
@@ -1457,6 +1472,7 @@ void llm_ctx_destroy(llm_ctx_t* c) {
     if (c->stage) (void)hipHostFree(c->stage);
     if (c->io_in) (void)hipHostFree(c->io_in);
     if (c->keys_host) (void)hipHostFree(c->keys_host);
+    if (c->probs.host) (void)hipHostFree(c->probs.host);
     for (auto e : c->gen_events) (void)hipEventDestroy(e);
     if (c->stream) (void)hipStreamDestroy(c->stream);
     delete c;
@@ -2724,6 +2740,154 @@ int llm_lm_head_argmax(llm_ctx_t* c, uint32_t pair, uint32_t row0, uint32_t rows
         tokens[r] = key_token(c->keys_host[r]);
         if (scores) scores[r] = key_score(c->keys_host[r]);
     }
+    return 0;
+}
+
+}  // extern "C"
+
+namespace {
+
+// Buffers of the probabilities and of the verification for the LM head.
+int ensure_probs(llm_ctx* c) {
+    llm_ctx::Probs& b = c->probs;
+    int rc;
+    if (!b.exp2) {
+        uint32_t* t = nullptr;
+        if ((rc = dev_alloc(c, (void**)&t, 2 * llm::kExp2Entries * 4))) return rc;
+        std::vector<uint32_t> h(2 * llm::kExp2Entries);
+        for (uint32_t i = 0; i < llm::kExp2Entries; i++) {
+            h[i] = (uint32_t)std::floor(std::exp2(30.0 - i / 1024.0) + 0.5);
+            h[llm::kExp2Entries + i] = (uint32_t)std::floor(std::exp2(30.0 - i / 1048576.0) + 0.5);
+        }
+        HIP_TRY(hipMemcpy(t, h.data(), h.size() * 4, hipMemcpyHostToDevice));
+        b.exp2 = t;
+    }
+    const size_t row = (size_t)8 * llm::kProbChunksMax;
+    if (!b.top && (rc = dev_alloc(c, (void**)&b.top, 8 * 8))) return rc;
+    if (!b.part && (rc = dev_alloc(c, (void**)&b.part, row * 8))) return rc;
+    if (!b.left && (rc = dev_alloc(c, (void**)&b.left, row * 16))) return rc;
+    if (!b.count && (rc = dev_alloc(c, (void**)&b.count, 9 * 32 * 4))) return rc;
+    if (!b.host &&
+        hipHostMalloc((void**)&b.host, 24 * sizeof(uint32_t), hipHostMallocDefault) != hipSuccess)
+        return fail(LLM_E_NOMEM, "hipHostMalloc failed");
+    const size_t lds = round_up(c->lm_vocab, 16);
+    if (b.lds < lds) {
+        int64_t* p = nullptr;
+        if ((rc = dev_alloc(c, (void**)&p, 8 * lds * 8))) return rc;
+        b.scores = p;
+        b.lds = lds;
+    }
+    return 0;
+}
+
+// log2(e) / temperature in units of 2^-24; 0: out of range.
+uint32_t inverse_temperature(double t) {
+    if (!(t >= 1.0 / 64 && t <= 64.0)) return 0;
+    return (uint32_t)std::floor(std::log2(std::exp(1.0)) / t * 16777216.0 + 0.5);
+}
+
+// The arguments that probabilities and verification share, checked.
+int check_lm_rows(llm_ctx* c, uint32_t pair, uint32_t row0, uint32_t rows, const char* what) {
+    if (!c || pair >= c->pairs.size() || rows == 0 || rows > 8 || row0 > 8 - rows)
+        return fail(LLM_E_ARG, std::string("bad ") + what + " arguments");
+    if (!c->lm_vocab) return fail(LLM_E_STATE, "LM head not loaded");
+    return 0;
+}
+
+// The rows' scores and largest scores enqueued; `a` filled but for the
+// temperatures.
+int enqueue_scores(llm_ctx* c, uint32_t pair, uint32_t row0, uint32_t rows, llm::ProbArgs& a) {
+    llm_ctx::Probs& b = c->probs;
+    a.scores = b.scores;
+    a.lds = (uint32_t)b.lds;
+    a.vocab = c->lm_vocab;
+    a.rows = rows;
+    a.exp2 = b.exp2;
+    a.keys = c->lm_keys;
+    a.top = b.top;
+    a.part = b.part;
+    c->busy = llm_ctx::WORK;
+    HIP_TRY(llm::launch_lm_scores(c->lm.d, c->lm.steps, c->lm_vocab,
+                                  c->pairs[pair] + (size_t)row0 * c->Hp, c->Hp, rows, c->lm.L,
+                                  c->lm_keys, b.scores, (uint32_t)b.lds, c->stream));
+    return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int llm_lm_head_probs(llm_ctx_t* c, uint32_t pair, uint32_t row0, uint32_t rows,
+                      const double* temperatures, uint32_t* probs) {
+    if (int rc = check_lm_rows(c, pair, row0, rows, "LM head probabilities")) return rc;
+    if (!temperatures || !probs || (uintptr_t)probs % 4)
+        return fail(LLM_E_ARG, "bad LM head probabilities arguments");
+    llm::ProbArgs a{};
+    for (uint32_t r = 0; r < rows; r++)
+        if ((a.inverse[r] = inverse_temperature(temperatures[r])) == 0)
+            return fail(LLM_E_ARG, "a temperature lies in [1/64, 64]");
+    HIP_TRY(hipSetDevice(c->device));
+    if (int rc = ensure_probs(c)) return rc;
+    if (int rc = enqueue_scores(c, pair, row0, rows, a)) return rc;
+    HIP_TRY(llm::launch_probs(a, probs, c->stream));
+    return 0;
+}
+
+int llm_lm_head_verify(llm_ctx_t* c, uint32_t pair, uint32_t row0, uint32_t requests,
+                       const uint32_t* draft_counts, const uint32_t* drafts,
+                       const uint32_t* accept_u, const uint32_t* sample_u,
+                       const double* temperatures, const uint32_t* draft_probs,
+                       uint32_t* accepted, uint32_t* tokens, uint32_t* probs) {
+    if (!c || requests == 0 || requests > 8 || !draft_counts || !sample_u || !temperatures ||
+        !accepted || !tokens || (uintptr_t)draft_probs % 4)
+        return fail(LLM_E_ARG, "bad LM head verification arguments");
+    llm::VerifyArgs a{};
+    uint32_t rows = 0, nd = 0;
+    for (uint32_t j = 0; j < requests; j++) {
+        if (draft_counts[j] > 7 || rows + draft_counts[j] + 1 > 8)
+            return fail(LLM_E_ARG, "drafts and requests are more than 8 rows");
+        a.first[j] = rows;
+        a.count[j] = draft_counts[j];
+        a.draft0[j] = nd;
+        rows += draft_counts[j] + 1;
+        nd += draft_counts[j];
+    }
+    if (nd && (!drafts || !accept_u))
+        return fail(LLM_E_ARG, "bad LM head verification arguments");
+    if (int rc = check_lm_rows(c, pair, row0, rows, "LM head verification")) return rc;
+    for (uint32_t j = 0; j < requests; j++) {
+        const uint32_t inv = inverse_temperature(temperatures[j]);
+        if (inv == 0) return fail(LLM_E_ARG, "a temperature lies in [1/64, 64]");
+        a.sample_u[j] = sample_u[j];
+        for (uint32_t i = 0; i <= a.count[j]; i++) {
+            const uint32_t r = a.first[j] + i;
+            a.p.inverse[r] = inv;
+            if (i == a.count[j]) break;
+            a.draft[r] = drafts[a.draft0[j] + i];
+            a.accept_u[r] = accept_u[a.draft0[j] + i];
+            if (a.draft[r] >= c->lm_vocab)
+                return fail(LLM_E_ARG, "drafted token " + std::to_string(a.draft[r]) +
+                                           " past the vocabulary");
+        }
+    }
+    HIP_TRY(hipSetDevice(c->device));
+    if (int rc = ensure_probs(c)) return rc;
+    if (int rc = enqueue_scores(c, pair, row0, rows, a.p)) return rc;
+    a.requests = requests;
+    a.q = nd ? draft_probs : nullptr;
+    a.left = c->probs.left;
+    a.count_in = c->probs.count;
+    a.host = c->probs.host;
+    a.flag = c->io_flag;
+    a.seq = ++c->io_seq;
+    HIP_TRY(llm::launch_verify(a, c->stream));
+    if (int rc = io_wait(c, a.seq)) return rc;
+    if (int rc = check_waits(c)) return rc;
+    for (uint32_t j = 0; j < requests; j++) {
+        accepted[j] = a.host[j];
+        tokens[j] = a.host[8 + j];
+    }
+    if (probs) std::memcpy(probs, a.host + 16, rows * sizeof(uint32_t));
     return 0;
 }
 

@@ -43,7 +43,7 @@ EXPORTS = (
     "llm_bench_projection", "llm_load_lm_head", "llm_lm_head_argmax",
     "llm_generate", "llm_lm_head_argmax_static", "llm_set_log",
     "llm_load_checkpoint_dir", "llm_op", "llm_port", "llm_port_write",
-    "llm_port_read", "llm_weight_bytes",
+    "llm_port_read", "llm_weight_bytes", "llm_lm_head_probs", "llm_lm_head_verify",
 )
 CKPT_TIE_EMBEDDINGS = 1
 CKPT_REQUIRE_LM_HEAD = 2
@@ -168,6 +168,12 @@ def load_library(path=LIB_PATH):
         "llm_port_read": (ctypes.c_int, [vp, _u32, _i16p, ctypes.c_size_t]),
         "llm_weight_bytes": (ctypes.c_int, [vp, ctypes.POINTER(ctypes.c_uint64),
                                             ctypes.POINTER(ctypes.c_uint32)]),
+        "llm_lm_head_probs": (ctypes.c_int, [vp, _u32, _u32, _u32,
+                                             ctypes.POINTER(ctypes.c_double), vp]),
+        "llm_lm_head_verify": (ctypes.c_int, [vp, _u32, _u32, _u32] +
+                               [ctypes.POINTER(_u32)] * 4 +
+                               [ctypes.POINTER(ctypes.c_double), vp] +
+                               [ctypes.POINTER(_u32)] * 3),
     }
     for name, (res, args) in sig.items():
         f = getattr(lib, name)
@@ -314,6 +320,34 @@ class Accelerator:
         self._check(lib().llm_lm_head_argmax(self._ctx, pair, row0, rows, toks,
                                              scores), "llm_lm_head_argmax")
         return list(toks), list(scores)
+
+    def lm_head_probs(self, pair, row0, temperatures, out_ptr):
+        """llm_lm_head_probs: Q0.32 next-token probabilities of one row per
+        temperature, rows row0 on, into device memory [rows][vocab] uint32 at
+        out_ptr.  Only enqueued on the context's stream."""
+        n = len(temperatures)
+        self._check(lib().llm_lm_head_probs(self._ctx, pair, row0, n,
+                                            (ctypes.c_double * n)(*temperatures), out_ptr),
+                    "llm_lm_head_probs")
+
+    def lm_head_verify(self, pair, row0, draft_counts, drafts, accept_u, sample_u,
+                       temperatures, draft_probs=None):
+        """llm_lm_head_verify: per request (draft_counts[j] drafts) the number
+        of drafts taken and the token drawn after them; also, per row, the
+        Q0.32 probability of its draft (a request's last row: of its drawn
+        token).  draft_probs: device address of [drafts][vocab] uint32, or
+        None where the drafter had no choice."""
+        n, nd = len(draft_counts), len(drafts)
+        rows = sum(draft_counts) + n
+        if nd != rows - n or len(accept_u) != nd or len(sample_u) != n or len(temperatures) != n:
+            raise AccelError("drafts, random numbers and requests do not match")
+        words = [(ctypes.c_uint32 * max(len(x), 1))(*x)
+                 for x in (draft_counts, drafts, accept_u, sample_u)]
+        accepted, tokens, probs = ((ctypes.c_uint32 * k)() for k in (n, n, max(rows, 1)))
+        self._check(lib().llm_lm_head_verify(
+            self._ctx, pair, row0, n, *words, (ctypes.c_double * max(n, 1))(*temperatures),
+            draft_probs, accepted, tokens, probs), "llm_lm_head_verify")
+        return list(accepted), list(tokens), list(probs)[:rows]
 
     def generate(self, embedding, prompt, block_size, layer_count, max_new_tokens,
                  log=None):
