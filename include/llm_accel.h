@@ -239,6 +239,32 @@ enum { LLM_PORT_IN = 0, LLM_PORT_AUX = 1, LLM_PORT_OUT = 2 };
 int llm_op(llm_ctx_t* ctx, uint32_t op, uint32_t layer, uint32_t token_count,
            uint32_t position, uint32_t tile_len, const int16_t* in,
            const int16_t* aux, int16_t* out, llm_status_t* status);
+/* No counterpart in the reference.  One of the seven projections (op 1-7 as
+ * in llm_op) of rows that belong to different requests, each under a low-rank
+ * adapter of its request: row r takes adapters[row_adapter[r]], or none where
+ * that is -1; rows that name the same adapter share its reads.  With x the
+ * row, W the loaded weights, rnd / sat as the projections narrow:
+ *   t_j = sat32(rnd(sum_k x_k a[j][k], 4)),
+ *   m_o = sat32(rnd(sum_j t_j b[j][o], 12)),
+ *   out_o = narrow(sum_k x_k W_ok + rnd(scale m_o, 12)),
+ * so a row without an adapter is llm_op's bit for bit.  a [rank][inputs] and
+ * b [rank][outputs] are device memory, row-major Q4.12, at 8-byte addresses,
+ * scale is Q16.16 (alpha / rank), rank 1..512; a and b are the caller's and
+ * must stay until the work is done.  `adapters` and `row_adapter`
+ * [token_count] are host memory, read before the call returns.  in and out
+ * are device memory as in llm_op (NULL: the context's ports; in at an 8-byte
+ * address; they may overlap).  Returns llm_op's status codes and counters;
+ * work is enqueued and not waited for.  The first call allocates. */
+typedef struct {
+    const int16_t* a;
+    const int16_t* b;
+    uint32_t rank;
+    int32_t scale;
+} llm_adapter_t;
+int llm_op_adapted(llm_ctx_t* ctx, uint32_t op, uint32_t layer, uint32_t token_count,
+                   const int16_t* in, int16_t* out, const llm_adapter_t* adapters,
+                   uint32_t adapter_count, const int32_t* row_adapter,
+                   llm_status_t* status);
 /* The context's port buffer `port` (device memory of *elems int16,
  * enough for every operator's tensor); allocated on first use.  Replaces
  * the reference host's six data buffers data_words_ (two per port name,

@@ -9,8 +9,9 @@ namespace llm {
 // Epilogues: STORE the narrowed sums; RESID add a residual row (and
 // optionally write a constant-gain RMSNorm of the result); SILU store
 // silu(gate) * up; STORE_NORM_IN like STORE on inputs normalised while they
-// are loaded (constant-gain RMSNorm of the raw rows).
-enum { EPI_STORE = 0, EPI_RESID = 1, EPI_SILU = 2, EPI_STORE_NORM_IN = 3 };
+// are loaded (constant-gain RMSNorm of the raw rows); WIDE stores the exact
+// sums themselves (ProjArgs::wide).
+enum { EPI_STORE = 0, EPI_RESID = 1, EPI_SILU = 2, EPI_STORE_NORM_IN = 3, EPI_WIDE = 4 };
 
 // Rows per weight block and columns per k-step of the "tile4x128" layout.
 constexpr uint32_t kBlockRows = 4;
@@ -74,6 +75,7 @@ struct ProjArgs {
     // copy holds the clamped value; unused words are 0.
     const uint32_t* corr0;
     const uint32_t* corr1;
+    int64_t* wide;  // EPI_WIDE: the sums [rows][ldo], 20 fraction bits
 };
 constexpr uint32_t kCorrSlots = 4;
 // Bytes of the p12 copy per 4-row block and k-step.

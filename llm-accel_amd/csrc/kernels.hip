@@ -1590,6 +1590,7 @@ hipError_t launch_proj(const ProjArgs& a, int epi, int L, uint32_t blocks,
         case EPI_STORE: return launch_mfma_epi<1, EPI_STORE>(a, st);
         case EPI_RESID: return launch_mfma_epi<1, EPI_RESID>(a, st);
         case EPI_STORE_NORM_IN: return launch_mfma_epi<1, EPI_STORE_NORM_IN>(a, st);
+        case EPI_WIDE: return launch_mfma_epi<1, EPI_WIDE>(a, st);
         default: return launch_mfma_epi<2, EPI_SILU>(a, st);
         }
     }
@@ -1597,6 +1598,7 @@ hipError_t launch_proj(const ProjArgs& a, int epi, int L, uint32_t blocks,
     case EPI_STORE: return launch_proj_epi<EPI_STORE>(a, L, blocks, st);
     case EPI_RESID: return launch_proj_epi<EPI_RESID>(a, L, blocks, st);
     case EPI_STORE_NORM_IN: return launch_proj_epi<EPI_STORE_NORM_IN>(a, L, blocks, st);
+    case EPI_WIDE: return launch_proj_epi<EPI_WIDE>(a, L, blocks, st);
     default: return launch_proj_epi<EPI_SILU>(a, L, blocks, st);
     }
 }

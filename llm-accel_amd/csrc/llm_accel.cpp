@@ -22,6 +22,7 @@
 #include <thread>
 #include <vector>
 
+#include "adapter.h"
 #include "attention.h"
 #include "coherent.h"
 #include "fixed_point.h"
@@ -227,6 +228,10 @@ struct llm_ctx {
     size_t port_n = 0;                  // elements per port
     int16_t* op_stage = nullptr;        // [8][max(Hp, Ip)]
     int32_t* op_tsum = nullptr;         // tile sums of the operator-level flash attention
+    // Projections with adapters (llm_op_adapted), allocated on first use: the
+    // exact sums [8][max(H, I)], and x A^T [8][kAdapterRankMax].
+    int64_t* op_wide = nullptr;
+    int32_t* op_t = nullptr;
     // partial sums / arrival counters of the split matrix-core projection
     int32_t* mf_part = nullptr;
     uint32_t* mf_count = nullptr;
@@ -1860,9 +1865,10 @@ void fill_op_counters(const llm_ctx* c, uint32_t op, uint32_t T, uint32_t pos,
 // and V are row ranges of the stored Q | K | V matrix.  The rows are
 // staged into 8 rows padded to whole k-steps: the projection kernels read
 // whole k-steps, and the matrix-core kernel all 8 rows (rows past T only
-// reach outputs that are not stored).
+// reach outputs that are not stored).  With `wide` the exact sums go there
+// instead, and `out` is not written.
 int enqueue_op_projection(llm_ctx* c, uint32_t layer, uint32_t proj, uint32_t T,
-                          const int16_t* in, int16_t* out) {
+                          const int16_t* in, int16_t* out, int64_t* wide = nullptr) {
     static const int mat_of[7] = {M_QKV, M_QKV, M_QKV, M_O, M_GATE, M_UP, M_DOWN};
     const Matrix& m = c->mat(layer, mat_of[proj]);
     const uint32_t row0 = proj == 1 ? c->H : proj == 2 ? c->H + c->Ckv : 0;
@@ -1872,7 +1878,7 @@ int enqueue_op_projection(llm_ctx* c, uint32_t layer, uint32_t proj, uint32_t T,
     // context's own port holds those where its tight rows are whole steps;
     // otherwise the rows are staged
     const bool direct = in == c->ports[LLM_PORT_IN] && m.k == m.k_pad &&
-                        (out + (size_t)T * n <= in || out >= in + c->port_n);
+                        (wide || out + (size_t)T * n <= in || out >= in + c->port_n);
     if (direct) {
     } else if (m.k % 8 == 0 && (uintptr_t)in % 16 == 0)  // what the copy kernel's loads need
         HIP_TRY(llm::launch_io_rows(in, m.k, c->op_stage, m.k_pad, m.k, T, nullptr, nullptr, 0,
@@ -1899,13 +1905,104 @@ int enqueue_op_projection(llm_ctx* c, uint32_t layer, uint32_t proj, uint32_t T,
         a.nc = (uint32_t)cdiv(n, llm::kMfRows);
     }
     if (m.corr_any) a.corr0 = m.corr + (size_t)row0 * llm::kCorrSlots;
-    HIP_TRY(llm::launch_proj(a, llm::EPI_STORE, m.L, (uint32_t)cdiv(n, 4), c->stream));
+    a.wide = wide;
+    HIP_TRY(llm::launch_proj(a, wide ? llm::EPI_WIDE : llm::EPI_STORE, m.L,
+                             (uint32_t)cdiv(n, 4), c->stream));
+    return 0;
+}
+
+// The rows of a command grouped by adapter, checked; rows without one are a
+// group of rank 0.
+int group_rows(uint32_t T, const llm_adapter_t* adapters, uint32_t count,
+               const int32_t* row_adapter, llm::AdapterArgs& a) {
+    int32_t of[8];
+    a.groups = a.ranks = 0;
+    for (uint32_t r = 0; r < T; r++) {
+        const int32_t id = row_adapter[r];
+        if (id < -1 || (id >= 0 && (uint32_t)id >= count))
+            return fail(LLM_E_ARG, "row " + std::to_string(r) + " names no adapter");
+        uint32_t g = 0;
+        while (g < a.groups && of[g] != id) g++;
+        llm::AdapterGroup& grp = a.g[g];
+        if (g == a.groups) {
+            grp = llm::AdapterGroup{};
+            if (id >= 0) {
+                const llm_adapter_t& ad = adapters[id];
+                if (!ad.a || !ad.b || ad.rank == 0 || ad.rank > llm::kAdapterRankMax ||
+                    (uintptr_t)ad.a % 8 || (uintptr_t)ad.b % 8)
+                    return fail(LLM_E_ARG, "adapter " + std::to_string(id) +
+                                               ": rank 1 to 512, factors at 8-byte addresses");
+                grp.a = ad.a;
+                grp.b = ad.b;
+                grp.rank = ad.rank;
+                grp.scale = ad.scale;
+                a.ranks += ad.rank;
+            }
+            of[a.groups++] = id;
+        }
+        grp.row[grp.rows++] = (uint8_t)r;
+    }
     return 0;
 }
 
 }  // namespace
 
 extern "C" {
+
+int llm_op_adapted(llm_ctx_t* c, uint32_t op, uint32_t layer, uint32_t token_count,
+                   const int16_t* in, int16_t* out, const llm_adapter_t* adapters,
+                   uint32_t adapter_count, const int32_t* row_adapter, llm_status_t* status) {
+    llm_status_t local;
+    llm_status_t* st = status ? status : &local;
+    std::memset(st, 0, sizeof(*st));
+    if (!c || (adapter_count && !adapters) || (token_count && !row_adapter))
+        return fail(LLM_E_ARG, "bad adapted projection arguments");
+    if (op < LLM_OP_Q_PROJECTION || op > LLM_OP_FFN_DOWN)
+        return fail(LLM_E_ARG, "operator " + std::to_string(op) + " is not a projection");
+    // as llm_op()
+    st->token_count = token_count;
+    st->last_task = 1;
+    auto reject = [&](uint32_t code) {
+        st->code = code;
+        return (int)code;
+    };
+    if (token_count > 8) return reject(LLM_STATUS_BAD_TOKEN_COUNT);
+    st->op = op;
+    if (layer >= c->L) return reject(LLM_STATUS_BAD_LAYER);
+    const uint32_t T = token_count, proj = op - 1;
+    llm::AdapterArgs a{};
+    if (int rc = group_rows(T, adapters, adapter_count, row_adapter, a)) return rc;
+    if ((uintptr_t)in % 8) return fail(LLM_E_ARG, "rows start at an 8-byte address");
+    HIP_TRY(hipSetDevice(c->device));
+    if (int rc = ensure_ports(c)) return rc;
+    if (!in) in = c->ports[LLM_PORT_IN];
+    if (!out) out = c->ports[LLM_PORT_OUT];
+    if (!c->loaded[layer * 7 + proj])
+        return fail(LLM_E_STATE, "layer " + std::to_string(layer) + " projection " +
+                                     std::to_string(proj) + " not loaded");
+    if (!c->op_wide)
+        if (int rc = dev_alloc(c, (void**)&c->op_wide, (size_t)8 * std::max(c->H, c->I) * 8))
+            return rc;
+    if (!c->op_t)
+        if (int rc = dev_alloc(c, (void**)&c->op_t, (size_t)8 * llm::kAdapterRankMax * 4))
+            return rc;
+    c->busy = llm_ctx::WORK;
+    if (T) {
+        if (int rc = enqueue_op_projection(c, layer, proj, T, in, out, c->op_wide)) return rc;
+        a.x = in;
+        a.inputs = op == LLM_OP_FFN_DOWN ? c->I : c->H;
+        a.outputs = op == LLM_OP_K_PROJECTION || op == LLM_OP_V_PROJECTION ? c->Ckv
+                    : op == LLM_OP_FFN_GATE || op == LLM_OP_FFN_UP         ? c->I
+                                                                           : c->H;
+        a.t = c->op_t;
+        a.wide = c->op_wide;
+        a.out = out;
+        HIP_TRY(llm::launch_adapter_in(a, c->stream));
+        HIP_TRY(llm::launch_adapter_out(a, c->stream));
+    }
+    fill_op_counters(c, op, T, 0, 0, st);
+    return LLM_STATUS_OK;
+}
 
 int llm_port(llm_ctx_t* c, uint32_t port, void** dev, size_t* elems) {
     if (!c || port > LLM_PORT_OUT) return fail(LLM_E_ARG, "bad port arguments");

@@ -171,6 +171,10 @@ __device__ __forceinline__ int64_t tree_sum64(F get) {
 template <int EPI, bool COH = false>
 __device__ __forceinline__ void proj_out(const ProjArgs& a, uint32_t r, uint32_t n,
                                          int64_t t0, int64_t t1, const EpiIn& ei) {
+    if (EPI == EPI_WIDE) {
+        a.wide[(size_t)r * a.ldo + n] = t0;
+        return;
+    }
     int16_t y = narrow16(t0);
     if (EPI == EPI_RESID) {
         y = sat16_32((int32_t)y + ei.res);

@@ -44,6 +44,7 @@ EXPORTS = (
     "llm_generate", "llm_lm_head_argmax_static", "llm_set_log",
     "llm_load_checkpoint_dir", "llm_op", "llm_port", "llm_port_write",
     "llm_port_read", "llm_weight_bytes", "llm_lm_head_probs", "llm_lm_head_verify",
+    "llm_op_adapted",
 )
 CKPT_TIE_EMBEDDINGS = 1
 CKPT_REQUIRE_LM_HEAD = 2
@@ -76,6 +77,13 @@ class Status(ctypes.Structure):
         return (self.op, self.code, self.token_count, self.output_waves,
                 self.mm_tasks, self.vector_tasks, self.completed_packets,
                 self.last_task)
+
+
+class Adapter(ctypes.Structure):
+    """llm_adapter_t: device addresses of a [rank][inputs] and b
+    [rank][outputs], the rank, and the scale in Q16.16."""
+    _fields_ = [("a", ctypes.c_void_p), ("b", ctypes.c_void_p),
+                ("rank", ctypes.c_uint32), ("scale", ctypes.c_int32)]
 
 
 class GenerateStats(ctypes.Structure):
@@ -168,6 +176,10 @@ def load_library(path=LIB_PATH):
         "llm_port_read": (ctypes.c_int, [vp, _u32, _i16p, ctypes.c_size_t]),
         "llm_weight_bytes": (ctypes.c_int, [vp, ctypes.POINTER(ctypes.c_uint64),
                                             ctypes.POINTER(ctypes.c_uint32)]),
+        "llm_op_adapted": (ctypes.c_int, [vp, _u32, _u32, _u32, vp, vp,
+                                          ctypes.POINTER(Adapter), _u32,
+                                          ctypes.POINTER(ctypes.c_int32),
+                                          ctypes.POINTER(Status)]),
         "llm_lm_head_probs": (ctypes.c_int, [vp, _u32, _u32, _u32,
                                              ctypes.POINTER(ctypes.c_double), vp]),
         "llm_lm_head_verify": (ctypes.c_int, [vp, _u32, _u32, _u32] +
@@ -422,6 +434,20 @@ class Accelerator:
             self.sync()
             return None, st
         return self.port_read(PORT_OUT, out_elems), st  # waits for the operator
+
+    def op_adapted(self, op, layer, row_adapter, adapters, in_ptr=None, out_ptr=None):
+        """llm_op_adapted: a projection of len(row_adapter) rows, row r under
+        adapters[row_adapter[r]] (-1: none), each adapter (a, b, rank, scale)
+        as in Adapter.  Rows and results are device memory, or the context's
+        in and out ports.  Only enqueued; returns the Status."""
+        st = Status()
+        n = len(row_adapter)
+        rc = lib().llm_op_adapted(
+            self._ctx, op, layer, n, in_ptr, out_ptr,
+            (Adapter * max(len(adapters), 1))(*(Adapter(*x) for x in adapters)), len(adapters),
+            (ctypes.c_int32 * max(n, 1))(*row_adapter), ctypes.byref(st))
+        self._check(rc, "llm_op_adapted")
+        return st
 
     def _checked(self, op, st):
         if st.code != STATUS_OK:
