@@ -265,6 +265,29 @@ int llm_op_adapted(llm_ctx_t* ctx, uint32_t op, uint32_t layer, uint32_t token_c
                    const int16_t* in, int16_t* out, const llm_adapter_t* adapters,
                    uint32_t adapter_count, const int32_t* row_adapter,
                    llm_status_t* status);
+/* No counterpart in the reference.  Attention of one query row per sequence
+ * for sequences that share their first prefix_len positions: those lie once
+ * in the cache of `layer`, each sequence's further positions in K / V rows of
+ * the caller's.  q and out are device memory [sequences][num_heads][d] (rows
+ * as the Q projection leaves them, after RoPE), k_own and v_own
+ * [sequences][num_kv_heads][own_capacity][d] (K after RoPE, V raw), own_len
+ * [sequences] the positions that each has (more than own_capacity count as
+ * own_capacity).  Row s is op 17's row of a cache that holds the prefix and
+ * then the sequence's own positions, bit for bit; a sequence with no position
+ * at all gets zeros.  Rows behind own_len are neither read nor written.
+ * 1..64 sequences, prefix_len <= max_seq_len, own_capacity <= 2^20 (0: k_own,
+ * v_own and own_len may be NULL); q, out, k_own and v_own start at 16-byte
+ * addresses; out may be q.  Work is enqueued and not waited for; own_len is
+ * read when it runs.  A call that needs more scratch than any before
+ * allocates (per query row and tile of 64 positions 136 + 2 d bytes); the
+ * scratch is the context's, so graphs that hold such calls must not run
+ * beside one another or beside the context's own work. */
+#define LLM_SHARED_SEQUENCES 64u
+#define LLM_SHARED_OWN_CAPACITY (1u << 20)
+int llm_attention_shared(llm_ctx_t* ctx, uint32_t layer, uint32_t prefix_len,
+                         uint32_t sequences, const int16_t* q, const int16_t* k_own,
+                         const int16_t* v_own, const uint32_t* own_len,
+                         uint32_t own_capacity, int16_t* out);
 /* The context's port buffer `port` (device memory of *elems int16,
  * enough for every operator's tensor); allocated on first use.  Replaces
  * the reference host's six data buffers data_words_ (two per port name,

@@ -29,6 +29,7 @@
 #include "kernels.h"
 #include "ops.h"
 #include "prefill.h"
+#include "shared_attention.h"
 #include "verify.h"
 
 namespace {
@@ -232,6 +233,10 @@ struct llm_ctx {
     // exact sums [8][max(H, I)], and x A^T [8][kAdapterRankMax].
     int64_t* op_wide = nullptr;
     int32_t* op_t = nullptr;
+    // Scratch of the shared-prefix attention, grown at least twofold; earlier
+    // ones stay the context's, for captured graphs that hold them.
+    uint8_t* shared_scratch = nullptr;
+    size_t shared_bytes = 0;
     // partial sums / arrival counters of the split matrix-core projection
     int32_t* mf_part = nullptr;
     uint32_t* mf_count = nullptr;
@@ -2002,6 +2007,55 @@ int llm_op_adapted(llm_ctx_t* c, uint32_t op, uint32_t layer, uint32_t token_cou
     }
     fill_op_counters(c, op, T, 0, 0, st);
     return LLM_STATUS_OK;
+}
+
+int llm_attention_shared(llm_ctx_t* c, uint32_t layer, uint32_t prefix, uint32_t sequences,
+                         const int16_t* q, const int16_t* k_own, const int16_t* v_own,
+                         const uint32_t* own_len, uint32_t own_capacity, int16_t* out) {
+    if (!c || layer >= c->L || !q || !out)
+        return fail(LLM_E_ARG, "bad shared attention arguments");
+    if (sequences == 0 || sequences > LLM_SHARED_SEQUENCES)
+        return fail(LLM_E_ARG, "1 to 64 sequences share a prefix");
+    if (prefix > c->max_seq) return fail(LLM_E_ARG, "prefix past the cache");
+    if (own_capacity > LLM_SHARED_OWN_CAPACITY)
+        return fail(LLM_E_ARG, "own_capacity past 2^20 positions");
+    if (own_capacity && (!k_own || !v_own || !own_len))
+        return fail(LLM_E_ARG, "bad shared attention arguments");
+    if ((uintptr_t)q % 16 || (uintptr_t)out % 16 ||
+        (own_capacity && ((uintptr_t)k_own % 16 || (uintptr_t)v_own % 16 || (uintptr_t)own_len % 4)))
+        return fail(LLM_E_ARG, "rows start at 16-byte addresses");
+    llm::SharedAttnArgs a{};
+    const size_t layer_off = (size_t)layer * c->Hkv * c->tiles * llm::kTile * c->d;
+    a.q = q;
+    a.kcache = c->kcache + layer_off;
+    a.vcache = c->vcache + layer_off;
+    a.pages = c->tiles;
+    a.k_own = k_own;
+    a.v_own = v_own;
+    a.own_len = own_len;
+    a.out = out;
+    a.sequences = sequences;
+    a.prefix = prefix;
+    a.own_cap = own_capacity;
+    a.kv_heads = c->Hkv;
+    a.group = c->G;
+    a.head_dim = c->d;
+    a.qk_scale = c->qk_scale;
+    a.exp14 = c->exp14;
+    llm::shared_attention_shape(a);
+    HIP_TRY(hipSetDevice(c->device));
+    const size_t need = llm::shared_attention_bytes(a);
+    if (c->shared_bytes < need) {
+        const size_t bytes = std::max(need, 2 * c->shared_bytes);
+        uint8_t* p = nullptr;
+        if (int rc = dev_alloc(c, (void**)&p, bytes)) return rc;
+        c->shared_scratch = p;
+        c->shared_bytes = bytes;
+    }
+    llm::shared_attention_scratch(a, c->shared_scratch);
+    c->busy = llm_ctx::WORK;
+    HIP_TRY(llm::launch_shared_attention(a, c->stream));
+    return 0;
 }
 
 int llm_port(llm_ctx_t* c, uint32_t port, void** dev, size_t* elems) {

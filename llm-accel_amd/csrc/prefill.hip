@@ -12,28 +12,13 @@
 #include "coherent.h"
 #include "fixed_point.h"
 #include "kernels.h"
+#include "mfma_common.h"
 #include "proj_common.h"
 
 namespace llm {
 namespace {
 
-typedef int32_t v4i __attribute__((ext_vector_type(4)));
 typedef int32_t v16i __attribute__((ext_vector_type(16)));
-
-__device__ __forceinline__ int32_t med3(int32_t v, int32_t lo, int32_t hi) {
-    return v < lo ? lo : (v > hi ? hi : v);
-}
-__device__ __forceinline__ uint32_t pack16(int32_t lo, int32_t hi) {
-    return ((uint32_t)lo & 0xffffu) | ((uint32_t)hi << 16);
-}
-// Byte planes of four int16 values (two packed words): c = x >> 8 and
-// d = (x & 255) - 128.
-__device__ __forceinline__ uint32_t plane_c(uint32_t w0, uint32_t w1) {
-    return __builtin_amdgcn_perm(w1, w0, 0x07050301u);
-}
-__device__ __forceinline__ uint32_t plane_d(uint32_t w0, uint32_t w1) {
-    return __builtin_amdgcn_perm(w1, w0, 0x06040200u) ^ 0x80808080u;
-}
 
 // ---------------------------------------------------------------------
 // Projection of many rows.  With x = 256 c + d + 128 (xp planes) and
@@ -760,34 +745,6 @@ __global__ __launch_bounds__(256) void pf_kvq_kernel(PfAttnArgs a, uint32_t ntil
     }
     const bool any = __syncthreads_or(extreme ? 1 : 0) != 0;
     if (tid == 0) a.qflag[head * mps + mp] = any ? 1u : 0u;
-}
-
-__device__ __forceinline__ v4i mfma16(v4i a, v4i b, v4i c) {
-    return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
-}
-// 1 in each byte whose (a, b) bytes are those of 2048 = 256 * 8 + 0.
-__device__ __forceinline__ v4i mask2048(v4i a, v4i b) {
-    v4i r;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const uint32_t z = ((uint32_t)a[i] ^ 0x08080808u) | (uint32_t)b[i];
-        const uint32_t nz = ((z & 0x7f7f7f7fu) + 0x7f7f7f7fu) | z;
-        r[i] = (int32_t)((~nz >> 7) & 0x01010101u);
-    }
-    return r;
-}
-// Maximum / sum over the four lanes l, l ^ 16, l ^ 32, l ^ 48.
-__device__ __forceinline__ int32_t quad_max(int32_t v) {
-    const auto p = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
-    v = max((int32_t)p[0], (int32_t)p[1]);
-    const auto q = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
-    return max((int32_t)q[0], (int32_t)q[1]);
-}
-__device__ __forceinline__ int32_t quad_sum(int32_t v) {
-    const auto p = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
-    v = (int32_t)p[0] + (int32_t)p[1];
-    const auto q = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
-    return (int32_t)q[0] + (int32_t)q[1];
 }
 
 // One workgroup per (32 rows, query head), tiles in sequence as the

@@ -44,7 +44,7 @@ EXPORTS = (
     "llm_generate", "llm_lm_head_argmax_static", "llm_set_log",
     "llm_load_checkpoint_dir", "llm_op", "llm_port", "llm_port_write",
     "llm_port_read", "llm_weight_bytes", "llm_lm_head_probs", "llm_lm_head_verify",
-    "llm_op_adapted",
+    "llm_op_adapted", "llm_attention_shared",
 )
 CKPT_TIE_EMBEDDINGS = 1
 CKPT_REQUIRE_LM_HEAD = 2
@@ -176,6 +176,7 @@ def load_library(path=LIB_PATH):
         "llm_port_read": (ctypes.c_int, [vp, _u32, _i16p, ctypes.c_size_t]),
         "llm_weight_bytes": (ctypes.c_int, [vp, ctypes.POINTER(ctypes.c_uint64),
                                             ctypes.POINTER(ctypes.c_uint32)]),
+        "llm_attention_shared": (ctypes.c_int, [vp, _u32, _u32, _u32, vp, vp, vp, vp, _u32, vp]),
         "llm_op_adapted": (ctypes.c_int, [vp, _u32, _u32, _u32, vp, vp,
                                           ctypes.POINTER(Adapter), _u32,
                                           ctypes.POINTER(ctypes.c_int32),
@@ -448,6 +449,15 @@ class Accelerator:
             (ctypes.c_int32 * max(n, 1))(*row_adapter), ctypes.byref(st))
         self._check(rc, "llm_op_adapted")
         return st
+
+    def attention_shared(self, layer, prefix_len, sequences, q_ptr, k_own_ptr, v_own_ptr,
+                         own_len_ptr, own_capacity, out_ptr):
+        """llm_attention_shared: attention of one query row per sequence over
+        the cache's first prefix_len positions and each sequence's own K / V
+        rows, all in device memory.  Only enqueued on the context's stream."""
+        self._check(lib().llm_attention_shared(
+            self._ctx, layer, prefix_len, sequences, q_ptr, k_own_ptr, v_own_ptr, own_len_ptr,
+            own_capacity, out_ptr), "llm_attention_shared")
 
     def _checked(self, op, st):
         if st.code != STATUS_OK:
