@@ -23,19 +23,20 @@ struct SharedAttnArgs {
     // then each sequence has up to own_tiles of its own (the first may begin
     // with the prefix's last positions); rows of a KV head are rho =
     // sequence * group + query head, padded to 16.
-    uint32_t whole, own_tiles, tiles, tmax_ld, rows, rows_pad;
+    uint32_t whole, own_tiles, tiles, rows, rows_pad;
     // scratch: scores, their maximum per tile, and per tile the factor of
     // what came before, the probabilities' sum, and the values
     int16_t* scores;  // [kv_heads][tiles][rows_pad][64]
-    int16_t* tmax;    // [kv_heads][rows_pad][tmax_ld]
+    int16_t* tmax;    // [kv_heads][tiles][rows_pad]
     int32_t* old;     // [kv_heads][tiles][rows_pad]
     int32_t* tsum;    // [kv_heads][tiles][rows_pad]
     int16_t* tval;    // [kv_heads][tiles][rows_pad][d]
-    // wavefronts of the launches over tiles: pieces of 16 rows per wavefront,
-    // such groups per shared tile, and the jobs
-    uint32_t per_wave, groups, shared_jobs, own_jobs;
+    uint32_t inv_group;  // 2^16 / group, rounded up: rho / group = rho inv_group >> 16
+    // workgroups of the launches over tiles: row groups per shared tile, and
+    // how many
+    uint32_t groups, shared_jobs, own_jobs;
 };
-// Fills the derived sizes (whole .. rows_pad, per_wave .. own_jobs).
+// Fills the derived sizes (whole .. own_jobs).
 void shared_attention_shape(SharedAttnArgs& a);
 // Bytes of the scratch, and its parts laid out from `base`.
 size_t shared_attention_bytes(const SharedAttnArgs& a);
