@@ -265,7 +265,7 @@ struct llm_ctx {
         int64_t* scores = nullptr;
         size_t lds = 0;
         uint32_t* exp2 = nullptr;
-        int64_t* top = nullptr;
+        llm::DrawPlace* place = nullptr;
         unsigned long long *part = nullptr, *left = nullptr;
         uint32_t* count = nullptr;
         uint32_t* host = nullptr;
@@ -2913,11 +2913,10 @@ int ensure_probs(llm_ctx* c) {
         HIP_TRY(hipMemcpy(t, h.data(), h.size() * 4, hipMemcpyHostToDevice));
         b.exp2 = t;
     }
-    const size_t row = (size_t)8 * llm::kProbChunksMax;
-    if (!b.top && (rc = dev_alloc(c, (void**)&b.top, 8 * 8))) return rc;
-    if (!b.part && (rc = dev_alloc(c, (void**)&b.part, row * 8))) return rc;
-    if (!b.left && (rc = dev_alloc(c, (void**)&b.left, row * 16))) return rc;
-    if (!b.count && (rc = dev_alloc(c, (void**)&b.count, 9 * 32 * 4))) return rc;
+    if (!b.place && (rc = dev_alloc(c, (void**)&b.place, 8 * sizeof(llm::DrawPlace)))) return rc;
+    if (!b.part && (rc = dev_alloc(c, (void**)&b.part, 8 * llm::kSumChunksMax * 8))) return rc;
+    if (!b.left && (rc = dev_alloc(c, (void**)&b.left, 8 * llm::kProbChunksMax * 16))) return rc;
+    if (!b.count && (rc = dev_alloc(c, (void**)&b.count, 17 * 32 * 4))) return rc;
     if (!b.host &&
         hipHostMalloc((void**)&b.host, 24 * sizeof(uint32_t), hipHostMallocDefault) != hipSuccess)
         return fail(LLM_E_NOMEM, "hipHostMalloc failed");
@@ -2955,8 +2954,9 @@ int enqueue_scores(llm_ctx* c, uint32_t pair, uint32_t row0, uint32_t rows, llm:
     a.rows = rows;
     a.exp2 = b.exp2;
     a.keys = c->lm_keys;
-    a.top = b.top;
     a.part = b.part;
+    a.place = b.place;
+    a.count_in = b.count;
     c->busy = llm_ctx::WORK;
     HIP_TRY(llm::launch_lm_scores(c->lm.d, c->lm.steps, c->lm_vocab,
                                   c->pairs[pair] + (size_t)row0 * c->Hp, c->Hp, rows, c->lm.L,
@@ -2974,9 +2974,12 @@ int llm_lm_head_probs(llm_ctx_t* c, uint32_t pair, uint32_t row0, uint32_t rows,
     if (!temperatures || !probs || (uintptr_t)probs % 4)
         return fail(LLM_E_ARG, "bad LM head probabilities arguments");
     llm::ProbArgs a{};
-    for (uint32_t r = 0; r < rows; r++)
+    a.requests = rows;  // without drafts
+    for (uint32_t r = 0; r < rows; r++) {
+        a.request[r] = a.first[r] = r;
         if ((a.inverse[r] = inverse_temperature(temperatures[r])) == 0)
             return fail(LLM_E_ARG, "a temperature lies in [1/64, 64]");
+    }
     HIP_TRY(hipSetDevice(c->device));
     if (int rc = ensure_probs(c)) return rc;
     if (int rc = enqueue_scores(c, pair, row0, rows, a)) return rc;
@@ -2992,7 +2995,7 @@ int llm_lm_head_verify(llm_ctx_t* c, uint32_t pair, uint32_t row0, uint32_t requ
     if (!c || requests == 0 || requests > 8 || !draft_counts || !sample_u || !temperatures ||
         !accepted || !tokens || (uintptr_t)draft_probs % 4)
         return fail(LLM_E_ARG, "bad LM head verification arguments");
-    llm::VerifyArgs a{};
+    llm::ProbArgs a{};
     uint32_t rows = 0, nd = 0;
     for (uint32_t j = 0; j < requests; j++) {
         if (draft_counts[j] > 7 || rows + draft_counts[j] + 1 > 8)
@@ -3012,7 +3015,8 @@ int llm_lm_head_verify(llm_ctx_t* c, uint32_t pair, uint32_t row0, uint32_t requ
         a.sample_u[j] = sample_u[j];
         for (uint32_t i = 0; i <= a.count[j]; i++) {
             const uint32_t r = a.first[j] + i;
-            a.p.inverse[r] = inv;
+            a.request[r] = j;
+            a.inverse[r] = inv;
             if (i == a.count[j]) break;
             a.draft[r] = drafts[a.draft0[j] + i];
             a.accept_u[r] = accept_u[a.draft0[j] + i];
@@ -3023,11 +3027,10 @@ int llm_lm_head_verify(llm_ctx_t* c, uint32_t pair, uint32_t row0, uint32_t requ
     }
     HIP_TRY(hipSetDevice(c->device));
     if (int rc = ensure_probs(c)) return rc;
-    if (int rc = enqueue_scores(c, pair, row0, rows, a.p)) return rc;
+    if (int rc = enqueue_scores(c, pair, row0, rows, a)) return rc;
     a.requests = requests;
     a.q = nd ? draft_probs : nullptr;
     a.left = c->probs.left;
-    a.count_in = c->probs.count;
     a.host = c->probs.host;
     a.flag = c->io_flag;
     a.seq = ++c->io_seq;

@@ -20,9 +20,10 @@
 //
 // The table of the LM head bounds a call (622 MB for 151,936 x 2,048: the
 // scores' pass reads it once and writes 8 bytes per score); what follows are
-// two short passes over the scores, one workgroup per 2,048 of them and row
-// (or request): the weights' sums, then the probabilities or the draws, the
-// last workgroup of a request to arrive drawing its token.
+// two short passes over the scores, a workgroup per chunk of them and row (or
+// request): the weights' sums, a request's last workgroup to arrive testing its
+// drafts, then the probabilities, or the draws, a request's last workgroup
+// drawing its token.
 #include "verify.h"
 
 #include "coherent.h"
@@ -98,133 +99,165 @@ __device__ __forceinline__ unsigned long long block_below64(unsigned long long v
     return s - v;
 }
 
-// Workgroup (chunk, row): the sum of the chunk's weights.
+// Q of a request's draft row i at token v.
+__device__ __forceinline__ uint32_t drafted(const ProbArgs& a, uint32_t j, uint32_t i,
+                                            uint32_t v) {
+    if (a.q) return a.q[(size_t)(a.draft0[j] + i) * a.vocab + v];
+    return v == a.draft[a.first[j] + i] ? 0xffffffffu : 0u;
+}
+
+// Workgroup (chunk, row): the sum of the chunk's weights.  The last one of a
+// request tests its drafts.
 __global__ __launch_bounds__(256) void prob_sums_kernel(ProbArgs a) {
     __shared__ __attribute__((aligned(16))) Exp2 e;
-    __shared__ unsigned long long red[4];
-    const uint32_t r = blockIdx.y, v0 = blockIdx.x * kProbChunk;
+    __shared__ unsigned long long red[4], total[8];
+    __shared__ uint32_t pdraft[8], taken[8], lds_last;
+    const uint32_t tid = threadIdx.x, r = blockIdx.y, v0 = blockIdx.x * kSumChunk;
+    const uint32_t chunks = gridDim.x, j = a.request[r], first = a.first[j], count = a.count[j];
+    const int64_t* s = a.scores + (size_t)r * a.lds;
+    constexpr uint32_t kEach = kSumChunk / 256;
+    int64_t sv[kEach];
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; i++) {
+        const uint32_t v = v0 + 256 * i + tid;
+        sv[i] = s[v < a.vocab ? v : 0];
+    }
     exp2_load(a.exp2, e);
     const int64_t top = (int64_t)(a.keys[r] >> 18) - ((int64_t)1 << 45);
     __syncthreads();
-    const int64_t* s = a.scores + (size_t)r * a.lds;
     const uint32_t c = a.inverse[r];
     unsigned long long sum = 0;
 #pragma unroll
-    for (uint32_t i = 0; i < kProbChunk / 256; i++) {
-        const uint32_t v = v0 + 256 * i + threadIdx.x;
-        if (v < a.vocab) sum += weight(e, top - s[v], c);
-    }
+    for (uint32_t i = 0; i < kEach; i++)
+        if (v0 + 256 * i + tid < a.vocab) sum += weight(e, top - sv[i], c);
     sum = block_sum64(sum, red);
-    if (threadIdx.x == 0) {
-        a.part[r * kProbChunksMax + blockIdx.x] = sum;
-        if (blockIdx.x == 0) a.top[r] = top;
-    }
-}
+    if (tid == 0) st_coherent(&a.part[r * kSumChunksMax + blockIdx.x], sum);
+    if (!arrive_last(a.count_in + 32 * r, chunks, &lds_last)) return;
+    if (count && !arrive_last(a.count_in + 32 * (8 + j), count + 1, &lds_last)) return;
 
-// The sum of row r's weights, by one wavefront (uniform over it).
-__device__ __forceinline__ uint64_t row_total(const ProbArgs& a, uint32_t r, uint32_t chunks) {
-    const uint32_t lane = threadIdx.x & 63;
-    unsigned long long z = 0;
-    for (uint32_t i = lane; i < chunks; i += 64) z += a.part[r * kProbChunksMax + i];
-    return wave_sum64(z);
+    // the rows' sums, a wavefront at a time
+    for (uint32_t i = tid >> 6; i <= count; i += 4) {
+        const uint32_t k = tid & 63;
+        const uint64_t z = wave_sum64(
+            k < chunks ? ld_coherent(&a.part[(first + i) * kSumChunksMax + k]) : 0);
+        if ((tid & 63) == 0) total[i] = z;
+    }
+    __syncthreads();
+    auto row_top = [&](uint32_t i) {
+        return (int64_t)(a.keys[first + i] >> 18) - ((int64_t)1 << 45);
+    };
+    if (tid < count) {
+        const uint32_t row = first + tid, x = a.draft[row];
+        const uint64_t z = total[tid];
+        const int64_t below = row_top(tid) - a.scores[(size_t)row * a.lds + x];
+        const uint32_t p = prob32(weight(e, below, a.inverse[row]), z, 1.0 / (double)z);
+        pdraft[tid] = p;
+        taken[tid] = (uint64_t)a.accept_u[row] * drafted(a, j, tid, x) < (uint64_t)p << 32;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        uint32_t at = 0;
+        while (at < count && taken[at]) at++;
+        DrawPlace* o = &a.place[j];
+        o->total = total[at];
+        o->top = row_top(at);
+        o->at = at;
+    }
+    if (tid < count) a.place[j].pdraft[tid] = pdraft[tid];
 }
 
 // Workgroup (chunk, row): the chunk's probabilities.
 __global__ __launch_bounds__(256) void probs_kernel(ProbArgs a, uint32_t* probs) {
     __shared__ __attribute__((aligned(16))) Exp2 e;
-    const uint32_t r = blockIdx.y, v0 = blockIdx.x * kProbChunk;
-    exp2_load(a.exp2, e);
-    const uint64_t z = row_total(a, r, gridDim.x);
-    const double inv = 1.0 / (double)z;
-    const int64_t top = a.top[r];
-    __syncthreads();
+    const uint32_t tid = threadIdx.x, r = blockIdx.y, v0 = blockIdx.x * kProbChunk;
     const int64_t* s = a.scores + (size_t)r * a.lds;
+    int64_t sv[kProbChunk / 256];
+#pragma unroll
+    for (uint32_t i = 0; i < kProbChunk / 256; i++) {
+        const uint32_t v = v0 + 256 * i + tid;
+        sv[i] = s[v < a.vocab ? v : 0];
+    }
+    exp2_load(a.exp2, e);
+    const uint64_t z = a.place[r].total;
+    const int64_t top = a.place[r].top;
+    const double inv = 1.0 / (double)z;
+    __syncthreads();
     const uint32_t c = a.inverse[r];
     uint32_t* out = probs + (size_t)r * a.vocab;
 #pragma unroll
     for (uint32_t i = 0; i < kProbChunk / 256; i++) {
-        const uint32_t v = v0 + 256 * i + threadIdx.x;
-        if (v < a.vocab) out[v] = prob32(weight(e, top - s[v], c), z, inv);
+        const uint32_t v = v0 + 256 * i + tid;
+        if (v < a.vocab) out[v] = prob32(weight(e, top - sv[i], c), z, inv);
     }
     // the keys are 0 between calls; nothing of this launch reads them
-    if (blockIdx.x == 0 && r == 0 && threadIdx.x < 8) a.keys[threadIdx.x] = 0;
+    if (blockIdx.x == 0 && r == 0 && tid < 8) a.keys[tid] = 0;
 }
 
-// Workgroup (chunk, request): the request's drafts tested, then the chunk's
-// part of the distribution its next token is drawn from; the request's last
-// workgroup draws it.
-__global__ __launch_bounds__(256) void verify_kernel(VerifyArgs a) {
+// Workgroup (chunk, request): the chunk's part of the distribution that the
+// request's next token is drawn from; its last workgroup draws it.
+__global__ __launch_bounds__(256) void draw_kernel(ProbArgs a) {
     __shared__ __attribute__((aligned(16))) Exp2 e;
-    __shared__ unsigned long long red[4];
-    __shared__ uint64_t total[8];
-    __shared__ uint32_t pdraft[8], taken[8], lds_last;
-    __shared__ unsigned long long before;
-    __shared__ uint32_t chunk;
-    const uint32_t tid = threadIdx.x, wave = tid >> 6, chunks = gridDim.x;
+    __shared__ unsigned long long red[4], before;
+    __shared__ uint32_t lds_last, chunk;
+    const uint32_t tid = threadIdx.x, chunks = gridDim.x;
     const uint32_t j = blockIdx.y, first = a.first[j], count = a.count[j];
-    exp2_load(a.p.exp2, e);
-    for (uint32_t i = wave; i <= count; i += 4) {
-        const uint64_t z = row_total(a.p, first + i, chunks);
-        if ((tid & 63) == 0) total[i] = z;
-    }
-    __syncthreads();
-    auto prob = [&](uint32_t i, uint32_t v) {  // P of the request's row i
-        const uint32_t r = first + i;
-        const uint64_t z = total[i];
-        return prob32(weight(e, a.p.top[r] - a.p.scores[(size_t)r * a.p.lds + v], a.p.inverse[r]),
-                      z, 1.0 / (double)z);
-    };
-    auto drafted = [&](uint32_t i, uint32_t v) -> uint32_t {  // Q
-        if (a.q) return a.q[(size_t)(a.draft0[j] + i) * a.p.vocab + v];
-        return v == a.draft[first + i] ? 0xffffffffu : 0u;
-    };
-    if (tid < count) {
-        const uint32_t x = a.draft[first + tid], p = prob(tid, x);
-        pdraft[tid] = p;
-        taken[tid] = (uint64_t)a.accept_u[first + tid] * drafted(tid, x) < (uint64_t)p << 32;
-    }
-    __syncthreads();
-    uint32_t at = 0;
-    while (at < count && taken[at]) at++;
-    // what is left of P where a token is drawn
-    auto above = [&](uint32_t p, uint32_t v) -> uint32_t {
-        if (at == count) return p;
-        const uint32_t q = drafted(at, v);
-        return p > q ? p - q : 0;
-    };
-    const uint32_t v0 = blockIdx.x * kProbChunk;
-    unsigned long long sl = 0, sp = 0;
-#pragma unroll 4
-    for (uint32_t i = 0; i < kProbChunk / 256; i++) {
-        const uint32_t v = v0 + 256 * i + tid;
-        if (v < a.p.vocab) {
-            const uint32_t p = prob(at, v);
-            sl += above(p, v);
-            sp += p;
+    const uint32_t at = a.place[j].at, row = first + at;
+    const uint64_t z = a.place[j].total;
+    const int64_t top = a.place[j].top;
+    const double inv = 1.0 / (double)z;
+    const int64_t* s = a.scores + (size_t)row * a.lds;
+    const uint32_t c = a.inverse[row];
+    constexpr uint32_t kEach = kProbChunk / 256;
+    // P of the thread's tokens of a chunk, and what of it lies above Q (`at`
+    // past the drafts: all of it)
+    uint32_t p[kEach], above[kEach];
+    auto fill = [&](uint32_t ch) {
+        const uint32_t v = ch * kProbChunk + kEach * tid;
+        int64_t sv[kEach];
+        uint32_t q[kEach];
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; i++) {
+            const uint32_t t = v + i;
+            sv[i] = s[t < a.vocab ? t : 0];
+            q[i] = at < count && t < a.vocab ? drafted(a, j, at, t) : 0;
         }
-    }
+        __syncthreads();  // (the tables, the first time)
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; i++) {
+            p[i] = 0;
+            if (v + i < a.vocab) p[i] = prob32(weight(e, top - sv[i], c), z, inv);
+            above[i] = p[i] > q[i] ? p[i] - q[i] : 0;
+        }
+    };
+    exp2_load(a.exp2, e);
+    fill(blockIdx.x);
+    unsigned long long sl = 0, sp = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; i++) sl += above[i], sp += p[i];
     sl = block_sum64(sl, red);
     sp = block_sum64(sp, red);
-    unsigned long long* left = a.left + (size_t)j * kProbChunksMax * 2;
-    if (tid == 0) {
-        st_coherent(&left[2 * blockIdx.x], sl);
-        st_coherent(&left[2 * blockIdx.x + 1], sp);
+    if (chunks > 1) {
+        unsigned long long* left = a.left + (size_t)j * kProbChunksMax * 2;
+        if (tid == 0) {
+            st_coherent(&left[2 * blockIdx.x], sl);
+            st_coherent(&left[2 * blockIdx.x + 1], sp);
+        }
+        if (!arrive_last(a.count_in + 32 * j, chunks, &lds_last)) return;
+        sl = sp = 0;
+        if (tid < chunks) {
+            sl = ld_coherent(&left[2 * tid]);
+            sp = ld_coherent(&left[2 * tid + 1]);
+        }
+    } else if (tid != 0) {
+        sl = sp = 0;
     }
-    if (!arrive_last(a.count_in + 32 * j, chunks, &lds_last)) return;
-
-    // ---- the draw ----
-    unsigned long long cl = 0, cp = 0;
-    if (tid < chunks) {
-        cl = ld_coherent(&left[2 * tid]);
-        cp = ld_coherent(&left[2 * tid + 1]);
-    }
-    const unsigned long long all_l = block_sum64(cl, red), all_p = block_sum64(cp, red);
+    const unsigned long long all_l = block_sum64(sl, red), all_p = block_sum64(sp, red);
     const bool whole = all_l == 0;  // nothing above Q: P itself
     const uint64_t sum = whole ? all_p : all_l;  // 1 .. 2^32
     const uint64_t t = ((uint64_t)a.sample_u[j] * sum) >> 32;
-    // the chunk, then the thread's scores of it, whose running sum passes t:
+    // the chunk, then the thread's tokens of it, whose running sum passes t:
     // one thread of the workgroup each time
-    const unsigned long long mass_c = whole ? cp : cl;
+    const unsigned long long mass_c = whole ? sp : sl;
     const unsigned long long below_c = block_below64(mass_c, red);
     if (t >= below_c && t < below_c + mass_c) {
         chunk = tid;
@@ -232,59 +265,63 @@ __global__ __launch_bounds__(256) void verify_kernel(VerifyArgs a) {
     }
     __syncthreads();
     const uint32_t ch = chunk;
-    // the chunk's scores, 8 in a row per thread
-    constexpr uint32_t kEach = kProbChunk / 256;
-    uint32_t mass[kEach], pv[kEach];
+    if (ch != blockIdx.x) fill(ch);
     unsigned long long mine = 0;
 #pragma unroll
     for (uint32_t i = 0; i < kEach; i++) {
-        const uint32_t v = ch * kProbChunk + kEach * tid + i;
-        mass[i] = pv[i] = 0;
-        if (v < a.p.vocab) {
-            pv[i] = prob(at, v);
-            mass[i] = whole ? pv[i] : above(pv[i], v);
-        }
-        mine += mass[i];
+        if (whole) above[i] = p[i];
+        mine += above[i];
     }
+    // the request's words reach the host (stores at system scope, each waited
+    // for) before its arrival, and all before the flag
+    auto tell = [&](uint32_t i, uint32_t v) {
+        __hip_atomic_store(a.host + i, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+    };
     uint64_t lower = before + block_below64(mine, red);
     if (t >= lower && t < lower + mine) {
-        uint32_t i = 0;
-        while (lower + mass[i] <= t) lower += mass[i++];
-        a.host[j] = at;
-        a.host[8 + j] = ch * kProbChunk + kEach * tid + i;
-        a.host[16 + first + count] = pv[i];
+        uint32_t at_i = 0, pv = p[0];
+#pragma unroll
+        for (uint32_t i = 0; i + 1 < kEach; i++)
+            if (at_i == i && lower + above[i] <= t) {
+                lower += above[i];
+                at_i = i + 1;
+                pv = p[i + 1];
+            }
+        tell(j, at);
+        tell(8 + j, ch * kProbChunk + kEach * tid + at_i);
+        tell(16 + first + count, pv);
     }
-    if (tid < count) a.host[16 + first + tid] = pdraft[tid];
-    // the request's words, then its arrival, reach the host before the flag
-    __threadfence_system();
+    if (tid < count) tell(16 + first + tid, a.place[j].pdraft[tid]);
+    __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
     if (tid != 0) return;
-    const uint32_t done = __hip_atomic_fetch_add(a.count_in + 32 * 8, 1u, __ATOMIC_ACQ_REL,
-                                                 __HIP_MEMORY_SCOPE_AGENT);
-    if (done != a.requests - 1) return;
-    __hip_atomic_store(a.count_in + 32 * 8, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    for (uint32_t r = 0; r < 8; r++) a.p.keys[r] = 0;  // nothing of this launch reads them
-    __hip_atomic_store(a.flag, a.seq, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_SYSTEM);
+    if (a.requests > 1) {
+        const uint32_t done = __hip_atomic_fetch_add(a.count_in + 32 * 16, 1u, __ATOMIC_RELAXED,
+                                                     __HIP_MEMORY_SCOPE_AGENT);
+        if (done != a.requests - 1) return;
+        __hip_atomic_store(a.count_in + 32 * 16, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    for (uint32_t r = 0; r < 8; r++) a.keys[r] = 0;  // nothing of this launch reads them
+    __hip_atomic_store(a.flag, a.seq, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
 }
 
-uint32_t chunks_of(const ProbArgs& a) { return (a.vocab + kProbChunk - 1) / kProbChunk; }
+uint32_t chunks_of(const ProbArgs& a, uint32_t each) { return (a.vocab + each - 1) / each; }
 
 }  // namespace
 
 hipError_t launch_probs(const ProbArgs& a, uint32_t* probs, hipStream_t st) {
-    const dim3 grid(chunks_of(a), a.rows);
-    prob_sums_kernel<<<grid, 256, 0, st>>>(a);
+    prob_sums_kernel<<<dim3(chunks_of(a, kSumChunk), a.rows), 256, 0, st>>>(a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    probs_kernel<<<grid, 256, 0, st>>>(a, probs);
+    probs_kernel<<<dim3(chunks_of(a, kProbChunk), a.rows), 256, 0, st>>>(a, probs);
     return hipGetLastError();
 }
 
-hipError_t launch_verify(const VerifyArgs& a, hipStream_t st) {
-    prob_sums_kernel<<<dim3(chunks_of(a.p), a.p.rows), 256, 0, st>>>(a.p);
+hipError_t launch_verify(const ProbArgs& a, hipStream_t st) {
+    prob_sums_kernel<<<dim3(chunks_of(a, kSumChunk), a.rows), 256, 0, st>>>(a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    verify_kernel<<<dim3(chunks_of(a.p), a.requests), 256, 0, st>>>(a);
+    draw_kernel<<<dim3(chunks_of(a, kProbChunk), a.requests), 256, 0, st>>>(a);
     return hipGetLastError();
 }
 

@@ -183,10 +183,7 @@ def load_library(path=LIB_PATH):
                                           ctypes.POINTER(Status)]),
         "llm_lm_head_probs": (ctypes.c_int, [vp, _u32, _u32, _u32,
                                              ctypes.POINTER(ctypes.c_double), vp]),
-        "llm_lm_head_verify": (ctypes.c_int, [vp, _u32, _u32, _u32] +
-                               [ctypes.POINTER(_u32)] * 4 +
-                               [ctypes.POINTER(ctypes.c_double), vp] +
-                               [ctypes.POINTER(_u32)] * 3),
+        "llm_lm_head_verify": (ctypes.c_int, [vp, _u32, _u32, _u32] + [vp] * 9),
     }
     for name, (res, args) in sig.items():
         f = getattr(lib, name)
@@ -354,13 +351,14 @@ class Accelerator:
         rows = sum(draft_counts) + n
         if nd != rows - n or len(accept_u) != nd or len(sample_u) != n or len(temperatures) != n:
             raise AccelError("drafts, random numbers and requests do not match")
-        words = [(ctypes.c_uint32 * max(len(x), 1))(*x)
-                 for x in (draft_counts, drafts, accept_u, sample_u)]
-        accepted, tokens, probs = ((ctypes.c_uint32 * k)() for k in (n, n, max(rows, 1)))
+        words = (ctypes.c_uint32 * (2 * n + 2 * nd))(*draft_counts, *drafts, *accept_u, *sample_u)
+        out = (ctypes.c_uint32 * (2 * n + rows))()  # accepted, tokens, probs
+        at = ctypes.byref
         self._check(lib().llm_lm_head_verify(
-            self._ctx, pair, row0, n, *words, (ctypes.c_double * max(n, 1))(*temperatures),
-            draft_probs, accepted, tokens, probs), "llm_lm_head_verify")
-        return list(accepted), list(tokens), list(probs)[:rows]
+            self._ctx, pair, row0, n, at(words), at(words, 4 * n), at(words, 4 * (n + nd)),
+            at(words, 4 * (n + 2 * nd)), (ctypes.c_double * n)(*temperatures), draft_probs,
+            at(out), at(out, 4 * n), at(out, 8 * n)), "llm_lm_head_verify")
+        return out[:n], out[n:2 * n], out[2 * n:]
 
     def generate(self, embedding, prompt, block_size, layer_count, max_new_tokens,
                  log=None):
