@@ -28,8 +28,8 @@ struct AdapterArgs {
     const int64_t* wide;  // the projection's exact sums [][outputs], 20 fraction bits
     int16_t* out;         // rows [][outputs], tight
 };
-// t = sat32(rnd(x A^T, 4)) of every row with an adapter.
-hipError_t launch_adapter_in(const AdapterArgs& a, hipStream_t st);
+// t = sat32(rnd(x A^T, 4)) of every row with an adapter: by workgroups of the
+// projection's own launch (EPI_WIDE, adapter_in.h).
 // out = narrow(wide + rnd(scale sat32(rnd(t B, 12)), 12)).
 hipError_t launch_adapter_out(const AdapterArgs& a, hipStream_t st);
 

@@ -4,6 +4,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "adapter.h"
+
 namespace llm {
 
 // Epilogues: STORE the narrowed sums; RESID add a residual row (and
@@ -76,6 +78,24 @@ struct ProjArgs {
     const uint32_t* corr0;
     const uint32_t* corr1;
     int64_t* wide;  // EPI_WIDE: the sums [rows][ldo], 20 fraction bits
+};
+// EPI_WIDE: rows past `rows` are not read (x may be a caller's memory), and
+// the workgroups past the projection's own `blocks` form x A^T of the rows'
+// adapters (adapter_in.h).
+struct ProjWideArgs : ProjArgs {
+    AdapterArgs ad;
+    uint32_t blocks;
+};
+// A kernel's argument by its epilogue.  (Specialised: an alias through an
+// expression of the enumerators enters the kernels' names, which host and
+// device compilation then spell differently.)
+template <int EPI>
+struct ArgsOf {
+    using type = ProjArgs;
+};
+template <>
+struct ArgsOf<EPI_WIDE> {
+    using type = ProjWideArgs;
 };
 constexpr uint32_t kCorrSlots = 4;
 // Bytes of the p12 copy per 4-row block and k-step.
@@ -151,6 +171,7 @@ bool proj_uses_mfma(const ProjArgs& a, int epi);
 // launch has one and K is at most kP12MaxSteps k-steps.
 constexpr uint32_t kP12MaxSteps = 128;
 bool proj_uses_p12(const ProjArgs& a, int epi);
+// (epi EPI_WIDE: `a` is a ProjWideArgs.)
 hipError_t launch_proj(const ProjArgs& a, int epi, int L, uint32_t blocks,
                        hipStream_t st);
 // RMSNorm of `rows` rows; const_gain > 0 selects the elementwise kernel

@@ -8,6 +8,7 @@
 //            [4 rows][16 lanes][8 columns].  One wavefront load of 16 B per
 //            lane reads one contiguous 1 KiB step of a block.  N is padded
 //            to a multiple of 4 and K to a multiple of 128 with zeros.
+#include "adapter_in.h"
 #include "kernels.h"
 
 #include "coherent.h"
@@ -121,8 +122,20 @@ __global__ __launch_bounds__(256) void rmsnorm_const_kernel(
 // loads (weights, activations, gammas) before the first product; loads past
 // its last step repeat that step (in bounds, products of zero).  SPW = 0:
 // a loop over the steps, LLM_PROJ_UNROLL steps of loads at a time.
+// Row r of the activations as a kernel of RT rows reads it: past the last
+// row those buffers hold rows that are not used, EPI_WIDE's repeat row 0.
+template <int EPI>
+__device__ __forceinline__ uint32_t row_in(const ProjArgs& a, uint32_t r) {
+    return EPI == EPI_WIDE && r >= a.rows ? 0 : r;
+}
 template <int RT, int L, int EPI, int WPB, int SPW>
-__global__ __launch_bounds__(64 * WPB) void proj_kernel(ProjArgs a) {
+__global__ __launch_bounds__(64 * WPB) void proj_kernel(typename ArgsOf<EPI>::type a) {
+    if constexpr (EPI == EPI_WIDE) {
+        if (blockIdx.x >= a.blocks) {
+            adapter_in_block<64 * WPB>(a.ad, blockIdx.x - a.blocks);
+            return;
+        }
+    }
     constexpr int NM = EPI == EPI_SILU ? 2 : 1;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int i = lane >> 4, j = lane & 15;
@@ -175,7 +188,7 @@ __global__ __launch_bounds__(64 * WPB) void proj_kernel(ProjArgs a) {
             } else {
 #pragma unroll
                 for (int r = 0; r < RT; r++)
-                    xv[u][r] = *(const uint4*)(xp + (size_t)r * a.ldx + du * 128);
+                    xv[u][r] = *(const uint4*)(xp + (size_t)row_in<EPI>(a, r) * a.ldx + du * 128);
             }
         }
         if constexpr (NIN) {
@@ -250,7 +263,7 @@ __global__ __launch_bounds__(64 * WPB) void proj_kernel(ProjArgs a) {
             uint4 xv[RT];
 #pragma unroll
             for (int r = 0; r < RT; r++)
-                xv[r] = *(const uint4*)(xp + (size_t)r * a.ldx);
+                xv[r] = *(const uint4*)(xp + (size_t)row_in<EPI>(a, r) * a.ldx);
             if (EPI == EPI_STORE_NORM_IN) {
                 // unconditional (the norm table is padded to whole k-steps):
                 // past in_cols the activations are 0 and so is the product
@@ -336,7 +349,13 @@ __global__ __launch_bounds__(64 * WPB) void proj_kernel(ProjArgs a) {
 // words are loaded when the kernel starts, a row's activations at its
 // correction columns in the epilogue, for rows that have any.
 template <int RT, int EPI, int WPB, int SPW, bool CORR = false>
-__global__ __launch_bounds__(64 * WPB) void proj_p12_kernel(ProjArgs a) {
+__global__ __launch_bounds__(64 * WPB) void proj_p12_kernel(typename ArgsOf<EPI>::type a) {
+    if constexpr (EPI == EPI_WIDE) {
+        if (blockIdx.x >= a.blocks) {
+            adapter_in_block<64 * WPB>(a.ad, blockIdx.x - a.blocks);
+            return;
+        }
+    }
     static_assert(SPW <= 32, "int32 partial sums");
     constexpr int NM = EPI == EPI_SILU ? 2 : 1;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -393,7 +412,7 @@ __global__ __launch_bounds__(64 * WPB) void proj_p12_kernel(ProjArgs a) {
         } else if constexpr (SPREAD) {
 #pragma unroll
             for (int r = 0; r < RT; r++)
-                xw[u][r] = *(const uint32_t*)(a.x + (size_t)r * a.ldx + (size_t)(s0 + du) * 128 + 2 * lane);
+                xw[u][r] = *(const uint32_t*)(a.x + (size_t)row_in<EPI>(a, r) * a.ldx + (size_t)(s0 + du) * 128 + 2 * lane);
         } else {
 #pragma unroll
             for (int r = 0; r < RT; r++) xv[u][r] = *(const uint4*)(xp + (size_t)r * a.ldx + du * 128);
@@ -764,7 +783,13 @@ __device__ __forceinline__ void mf_finish(const ProjArgs& a, uint32_t c, uint32_
 }
 
 template <int NM, int KS, int QM, int PD, int EPI>
-__global__ __launch_bounds__(64 * KS) void proj_mfma_kernel(ProjArgs a, uint32_t parts) {
+__global__ __launch_bounds__(64 * KS) void proj_mfma_kernel(typename ArgsOf<EPI>::type a, uint32_t parts) {
+    if constexpr (EPI == EPI_WIDE) {
+        if (blockIdx.x >= a.blocks) {
+            adapter_in_block<64 * KS>(a.ad, blockIdx.x - a.blocks);
+            return;
+        }
+    }
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint32_t c = blockIdx.x / parts, p = blockIdx.x % parts, KQ = a.kq;
     const uint32_t pq0 = p * KQ / parts, pq1 = (p + 1) * KQ / parts;
@@ -773,9 +798,11 @@ __global__ __launch_bounds__(64 * KS) void proj_mfma_kernel(ProjArgs a, uint32_t
     const uint32_t n = q1 - q0;  // <= QM (the launcher's choice)
     const uint32_t i = lane & 15, g = lane >> 4;
     const bool hi_plane = i < 8;
-    // every activation buffer holds 8 rows: row i & 7 is always in bounds;
-    // lane i holds inputs 8 (i / 8) .. + 7 of its 16
-    const int16_t* xp = a.x + (size_t)(i & 7) * a.ldx + 16 * g + 8 * (i >> 3);
+    // every activation buffer holds 8 rows: row i & 7 is always in bounds (but
+    // EPI_WIDE's: rows past the last repeat it); lane i holds inputs 8 (i / 8)
+    // .. + 7 of its 16
+    const uint32_t xr = EPI == EPI_WIDE ? min(i & 7, a.rows - 1) : i & 7;
+    const int16_t* xp = a.x + (size_t)xr * a.ldx + 16 * g + 8 * (i >> 3);
     const int16_t* gp = EPI == EPI_STORE_NORM_IN ? a.in_gamma + 16 * g + 8 * (i >> 3) : nullptr;
     const MfEpi<NM, EPI> fe = mf_epi_fetch<NM, EPI>(a, c);
     const int8_t* bp[NM];
@@ -854,7 +881,13 @@ __device__ __forceinline__ void p12_step_load(const ProjArgs& a, const uint8_t* 
 }
 
 template <int NM, int KS, int SM, int PDS, int EPI>
-__global__ __launch_bounds__(64 * KS) void proj_mfma12_kernel(ProjArgs a, uint32_t parts) {
+__global__ __launch_bounds__(64 * KS) void proj_mfma12_kernel(typename ArgsOf<EPI>::type a, uint32_t parts) {
+    if constexpr (EPI == EPI_WIDE) {
+        if (blockIdx.x >= a.blocks) {
+            adapter_in_block<64 * KS>(a.ad, blockIdx.x - a.blocks);
+            return;
+        }
+    }
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint32_t c = blockIdx.x / parts, p = blockIdx.x % parts, S = a.steps, KQ = a.kq;
     const uint32_t ps0 = p * S / parts, ps1 = (p + 1) * S / parts;
@@ -863,7 +896,8 @@ __global__ __launch_bounds__(64 * KS) void proj_mfma12_kernel(ProjArgs a, uint32
     const uint32_t n = s1 - s0;  // <= SM (the launcher's choice)
     const uint32_t i = lane & 15, g = lane >> 4;
     const bool hi_plane = i < 8;
-    const int16_t* xp = a.x + (size_t)(i & 7) * a.ldx + 16 * g + 8 * (i >> 3);
+    const uint32_t xr = EPI == EPI_WIDE ? min(i & 7, a.rows - 1) : i & 7;
+    const int16_t* xp = a.x + (size_t)xr * a.ldx + 16 * g + 8 * (i >> 3);
     const int16_t* gp = EPI == EPI_STORE_NORM_IN ? a.in_gamma + 16 * g + 8 * (i >> 3) : nullptr;
     const MfEpi<NM, EPI> fe = mf_epi_fetch<NM, EPI>(a, c);
     // load lanes: block 4c + lane / 16, clamped to the copy's last block
@@ -1366,13 +1400,32 @@ __global__ __launch_bounds__(256) void copy_kernel(const uint4* __restrict__ src
 // ---------------------------------------------------------------------
 // launchers
 // ---------------------------------------------------------------------
+// The launch's arguments and grid: EPI_WIDE's carry the adapters and, past the
+// projection's `blocks`, the workgroups of x A^T.
+template <int EPI>
+static typename ArgsOf<EPI>::type args_of(const ProjArgs& a, uint32_t blocks) {
+    if constexpr (EPI == EPI_WIDE) {
+        ProjWideArgs w = static_cast<const ProjWideArgs&>(a);
+        w.blocks = blocks;
+        return w;
+    } else {
+        (void)blocks;
+        return a;
+    }
+}
+template <int EPI>
+static uint32_t grid_of(const ProjArgs& a, uint32_t blocks) {
+    if constexpr (EPI == EPI_WIDE) blocks += static_cast<const ProjWideArgs&>(a).ad.ranks;
+    return blocks;
+}
+
 template <int RT, int EPI, int W, int SPW>
 static void launch_proj_s(const ProjArgs& a, int L, uint32_t blocks, hipStream_t st) {
     // SPW <= 4: with L >= 4 the int32 sums of a wavefront's steps widen
     // once at the end; L 1..3 widens after every step, L 0 every product
-    if (L >= 4) proj_kernel<RT, 4, EPI, W, SPW><<<blocks, 64 * W, 0, st>>>(a);
-    else if (L >= 1) proj_kernel<RT, 1, EPI, W, SPW><<<blocks, 64 * W, 0, st>>>(a);
-    else proj_kernel<RT, 0, EPI, W, SPW><<<blocks, 64 * W, 0, st>>>(a);
+    if (L >= 4) proj_kernel<RT, 4, EPI, W, SPW><<<grid_of<EPI>(a, blocks), 64 * W, 0, st>>>(args_of<EPI>(a, blocks));
+    else if (L >= 1) proj_kernel<RT, 1, EPI, W, SPW><<<grid_of<EPI>(a, blocks), 64 * W, 0, st>>>(args_of<EPI>(a, blocks));
+    else proj_kernel<RT, 0, EPI, W, SPW><<<grid_of<EPI>(a, blocks), 64 * W, 0, st>>>(args_of<EPI>(a, blocks));
 }
 
 template <int RT, int EPI, int W>
@@ -1388,11 +1441,11 @@ static hipError_t launch_proj_w(const ProjArgs& a, int L, uint32_t blocks,
         return hipGetLastError();
     }
     switch (L) {
-    case 0: proj_kernel<RT, 0, EPI, W, 0><<<blocks, 64 * W, 0, st>>>(a); break;
-    case 1: proj_kernel<RT, 1, EPI, W, 0><<<blocks, 64 * W, 0, st>>>(a); break;
-    case 4: proj_kernel<RT, 4, EPI, W, 0><<<blocks, 64 * W, 0, st>>>(a); break;
-    case 8: proj_kernel<RT, 8, EPI, W, 0><<<blocks, 64 * W, 0, st>>>(a); break;
-    default: proj_kernel<RT, 16, EPI, W, 0><<<blocks, 64 * W, 0, st>>>(a); break;
+    case 0: proj_kernel<RT, 0, EPI, W, 0><<<grid_of<EPI>(a, blocks), 64 * W, 0, st>>>(args_of<EPI>(a, blocks)); break;
+    case 1: proj_kernel<RT, 1, EPI, W, 0><<<grid_of<EPI>(a, blocks), 64 * W, 0, st>>>(args_of<EPI>(a, blocks)); break;
+    case 4: proj_kernel<RT, 4, EPI, W, 0><<<grid_of<EPI>(a, blocks), 64 * W, 0, st>>>(args_of<EPI>(a, blocks)); break;
+    case 8: proj_kernel<RT, 8, EPI, W, 0><<<grid_of<EPI>(a, blocks), 64 * W, 0, st>>>(args_of<EPI>(a, blocks)); break;
+    default: proj_kernel<RT, 16, EPI, W, 0><<<grid_of<EPI>(a, blocks), 64 * W, 0, st>>>(args_of<EPI>(a, blocks)); break;
     }
     return hipGetLastError();
 }
@@ -1418,10 +1471,10 @@ static void launch_p12_c(const ProjArgs& a, uint32_t blocks, hipStream_t st) {
     const uint32_t spw = (a.steps + W - 1) / W;
     // the smallest variant that holds the steps (registers decide how many
     // 16-wavefront blocks a compute unit holds)
-    if (spw <= 2) proj_p12_kernel<RT, EPI, W, 2, CORR><<<blocks, 64 * W, 0, st>>>(a);
-    else if (spw <= 4) proj_p12_kernel<RT, EPI, W, 4, CORR><<<blocks, 64 * W, 0, st>>>(a);
-    else if (spw <= 6) proj_p12_kernel<RT, EPI, W, 6, CORR><<<blocks, 64 * W, 0, st>>>(a);
-    else proj_p12_kernel<RT, EPI, W, 8, CORR><<<blocks, 64 * W, 0, st>>>(a);
+    if (spw <= 2) proj_p12_kernel<RT, EPI, W, 2, CORR><<<grid_of<EPI>(a, blocks), 64 * W, 0, st>>>(args_of<EPI>(a, blocks));
+    else if (spw <= 4) proj_p12_kernel<RT, EPI, W, 4, CORR><<<grid_of<EPI>(a, blocks), 64 * W, 0, st>>>(args_of<EPI>(a, blocks));
+    else if (spw <= 6) proj_p12_kernel<RT, EPI, W, 6, CORR><<<grid_of<EPI>(a, blocks), 64 * W, 0, st>>>(args_of<EPI>(a, blocks));
+    else proj_p12_kernel<RT, EPI, W, 8, CORR><<<grid_of<EPI>(a, blocks), 64 * W, 0, st>>>(args_of<EPI>(a, blocks));
 }
 template <int RT, int EPI, int W>
 static hipError_t launch_p12_w(const ProjArgs& a, uint32_t blocks, hipStream_t st) {
@@ -1480,7 +1533,8 @@ template <int NM, int KS, int QM, int EPI>
 static void launch_mfma_k(const ProjArgs& a, uint32_t parts, hipStream_t st) {
     constexpr int PD0 = NM == 2 ? LLM_MF_PD2 : LLM_MF_PD1;
     constexpr int PD = PD0 < QM ? PD0 : QM;
-    proj_mfma_kernel<NM, KS, QM, PD, EPI><<<a.nc * parts, 64 * KS, 0, st>>>(a, parts);
+    proj_mfma_kernel<NM, KS, QM, PD, EPI><<<grid_of<EPI>(a, a.nc * parts), 64 * KS, 0, st>>>(
+        args_of<EPI>(a, a.nc * parts), parts);
 }
 
 template <int NM, int KS, int EPI>
@@ -1530,7 +1584,8 @@ static void launch_mfma12_k(const ProjArgs& a, uint32_t parts, hipStream_t st) {
     // normalising on load holds the gammas too: one step in flight
     constexpr int PD0 = NM == 2 ? LLM_MF12_PD2 : EPI == EPI_STORE_NORM_IN ? 1 : LLM_MF12_PD1;
     constexpr int PD = PD0 < SM ? PD0 : SM;
-    proj_mfma12_kernel<NM, KS, SM, PD, EPI><<<a.nc * parts, 64 * KS, 0, st>>>(a, parts);
+    proj_mfma12_kernel<NM, KS, SM, PD, EPI><<<grid_of<EPI>(a, a.nc * parts), 64 * KS, 0, st>>>(
+        args_of<EPI>(a, a.nc * parts), parts);
 }
 
 template <int NM, int KS, int EPI>

@@ -1870,10 +1870,10 @@ void fill_op_counters(const llm_ctx* c, uint32_t op, uint32_t T, uint32_t pos,
 // and V are row ranges of the stored Q | K | V matrix.  The rows are
 // staged into 8 rows padded to whole k-steps: the projection kernels read
 // whole k-steps, and the matrix-core kernel all 8 rows (rows past T only
-// reach outputs that are not stored).  With `wide` the exact sums go there
-// instead, and `out` is not written.
+// reach outputs that are not stored).  With adapters (their groups set) the
+// exact sums and x A^T go to the context's scratch, and then all to out.
 int enqueue_op_projection(llm_ctx* c, uint32_t layer, uint32_t proj, uint32_t T,
-                          const int16_t* in, int16_t* out, int64_t* wide = nullptr) {
+                          const int16_t* in, int16_t* out, llm::AdapterArgs* ad = nullptr) {
     static const int mat_of[7] = {M_QKV, M_QKV, M_QKV, M_O, M_GATE, M_UP, M_DOWN};
     const Matrix& m = c->mat(layer, mat_of[proj]);
     const uint32_t row0 = proj == 1 ? c->H : proj == 2 ? c->H + c->Ckv : 0;
@@ -1882,8 +1882,11 @@ int enqueue_op_projection(llm_ctx* c, uint32_t layer, uint32_t proj, uint32_t T,
     // the kernels read whole k-steps and, for 3 rows on, all 8 rows: the
     // context's own port holds those where its tight rows are whole steps;
     // otherwise the rows are staged
-    const bool direct = in == c->ports[LLM_PORT_IN] && m.k == m.k_pad &&
-                        (wide || out + (size_t)T * n <= in || out >= in + c->port_n);
+    // (and a launch with adapters reads no row past the last)
+    const bool direct = m.k == m.k_pad &&
+                        (ad ? (uintptr_t)in % 16 == 0
+                            : in == c->ports[LLM_PORT_IN] &&
+                                  (out + (size_t)T * n <= in || out >= in + c->port_n));
     if (direct) {
     } else if (m.k % 8 == 0 && (uintptr_t)in % 16 == 0)  // what the copy kernel's loads need
         HIP_TRY(llm::launch_io_rows(in, m.k, c->op_stage, m.k_pad, m.k, T, nullptr, nullptr, 0,
@@ -1891,7 +1894,7 @@ int enqueue_op_projection(llm_ctx* c, uint32_t layer, uint32_t proj, uint32_t T,
     else
         HIP_TRY(hipMemcpy2DAsync(c->op_stage, (size_t)m.k_pad * 2, in, (size_t)m.k * 2,
                                  (size_t)m.k * 2, T, hipMemcpyDeviceToDevice, c->stream));
-    llm::ProjArgs a{};
+    llm::ProjWideArgs a{};
     a.w0 = m.d ? m.d + (size_t)row0 * m.k_pad : nullptr;
     a.steps = m.steps;
     a.x = direct ? in : c->op_stage;
@@ -1910,9 +1913,19 @@ int enqueue_op_projection(llm_ctx* c, uint32_t layer, uint32_t proj, uint32_t T,
         a.nc = (uint32_t)cdiv(n, llm::kMfRows);
     }
     if (m.corr_any) a.corr0 = m.corr + (size_t)row0 * llm::kCorrSlots;
-    a.wide = wide;
-    HIP_TRY(llm::launch_proj(a, wide ? llm::EPI_WIDE : llm::EPI_STORE, m.L,
-                             (uint32_t)cdiv(n, 4), c->stream));
+    if (!ad) {
+        HIP_TRY(llm::launch_proj(a, llm::EPI_STORE, m.L, (uint32_t)cdiv(n, 4), c->stream));
+        return 0;
+    }
+    ad->x = in;
+    ad->inputs = m.k;
+    ad->outputs = n;
+    ad->wide = a.wide = c->op_wide;
+    ad->t = c->op_t;
+    ad->out = out;
+    a.ad = *ad;
+    HIP_TRY(llm::launch_proj(a, llm::EPI_WIDE, m.L, (uint32_t)cdiv(n, 4), c->stream));
+    HIP_TRY(llm::launch_adapter_out(*ad, c->stream));
     return 0;
 }
 
@@ -1992,19 +2005,7 @@ int llm_op_adapted(llm_ctx_t* c, uint32_t op, uint32_t layer, uint32_t token_cou
         if (int rc = dev_alloc(c, (void**)&c->op_t, (size_t)8 * llm::kAdapterRankMax * 4))
             return rc;
     c->busy = llm_ctx::WORK;
-    if (T) {
-        if (int rc = enqueue_op_projection(c, layer, proj, T, in, out, c->op_wide)) return rc;
-        a.x = in;
-        a.inputs = op == LLM_OP_FFN_DOWN ? c->I : c->H;
-        a.outputs = op == LLM_OP_K_PROJECTION || op == LLM_OP_V_PROJECTION ? c->Ckv
-                    : op == LLM_OP_FFN_GATE || op == LLM_OP_FFN_UP         ? c->I
-                                                                           : c->H;
-        a.t = c->op_t;
-        a.wide = c->op_wide;
-        a.out = out;
-        HIP_TRY(llm::launch_adapter_in(a, c->stream));
-        HIP_TRY(llm::launch_adapter_out(a, c->stream));
-    }
+    if (int rc = enqueue_op_projection(c, layer, proj, T, in, out, &a)) return rc;
     fill_op_counters(c, op, T, 0, 0, st);
     return LLM_STATUS_OK;
 }

@@ -443,7 +443,7 @@ class Accelerator:
         n = len(row_adapter)
         rc = lib().llm_op_adapted(
             self._ctx, op, layer, n, in_ptr, out_ptr,
-            (Adapter * max(len(adapters), 1))(*(Adapter(*x) for x in adapters)), len(adapters),
+            (Adapter * max(len(adapters), 1))(*adapters), len(adapters),
             (ctypes.c_int32 * max(n, 1))(*row_adapter), ctypes.byref(st))
         self._check(rc, "llm_op_adapted")
         return st
