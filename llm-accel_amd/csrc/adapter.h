@@ -22,6 +22,7 @@ struct AdapterArgs {
     AdapterGroup g[8];
     uint32_t groups;
     uint32_t ranks;       // of all groups together
+    uint32_t start[8];    // ranks of the groups before each (no group: ~0)
     const int16_t* x;     // rows [][inputs], tight
     uint32_t inputs, outputs;
     int32_t* t;           // [8][kAdapterRankMax] Q16.16: x A^T

@@ -1414,8 +1414,11 @@ static typename ArgsOf<EPI>::type args_of(const ProjArgs& a, uint32_t blocks) {
     }
 }
 template <int EPI>
-static uint32_t grid_of(const ProjArgs& a, uint32_t blocks) {
-    if constexpr (EPI == EPI_WIDE) blocks += static_cast<const ProjWideArgs&>(a).ad.ranks;
+static uint32_t grid_of(const ProjArgs& a, uint32_t blocks, uint32_t threads) {
+    if constexpr (EPI == EPI_WIDE) {
+        const uint32_t columns = threads / kInThreads;  // of a workgroup
+        blocks += (static_cast<const ProjWideArgs&>(a).ad.ranks + columns - 1) / columns;
+    }
     return blocks;
 }
 
@@ -1423,9 +1426,9 @@ template <int RT, int EPI, int W, int SPW>
 static void launch_proj_s(const ProjArgs& a, int L, uint32_t blocks, hipStream_t st) {
     // SPW <= 4: with L >= 4 the int32 sums of a wavefront's steps widen
     // once at the end; L 1..3 widens after every step, L 0 every product
-    if (L >= 4) proj_kernel<RT, 4, EPI, W, SPW><<<grid_of<EPI>(a, blocks), 64 * W, 0, st>>>(args_of<EPI>(a, blocks));
-    else if (L >= 1) proj_kernel<RT, 1, EPI, W, SPW><<<grid_of<EPI>(a, blocks), 64 * W, 0, st>>>(args_of<EPI>(a, blocks));
-    else proj_kernel<RT, 0, EPI, W, SPW><<<grid_of<EPI>(a, blocks), 64 * W, 0, st>>>(args_of<EPI>(a, blocks));
+    if (L >= 4) proj_kernel<RT, 4, EPI, W, SPW><<<grid_of<EPI>(a, blocks, 64 * W), 64 * W, 0, st>>>(args_of<EPI>(a, blocks));
+    else if (L >= 1) proj_kernel<RT, 1, EPI, W, SPW><<<grid_of<EPI>(a, blocks, 64 * W), 64 * W, 0, st>>>(args_of<EPI>(a, blocks));
+    else proj_kernel<RT, 0, EPI, W, SPW><<<grid_of<EPI>(a, blocks, 64 * W), 64 * W, 0, st>>>(args_of<EPI>(a, blocks));
 }
 
 template <int RT, int EPI, int W>
@@ -1441,11 +1444,11 @@ static hipError_t launch_proj_w(const ProjArgs& a, int L, uint32_t blocks,
         return hipGetLastError();
     }
     switch (L) {
-    case 0: proj_kernel<RT, 0, EPI, W, 0><<<grid_of<EPI>(a, blocks), 64 * W, 0, st>>>(args_of<EPI>(a, blocks)); break;
-    case 1: proj_kernel<RT, 1, EPI, W, 0><<<grid_of<EPI>(a, blocks), 64 * W, 0, st>>>(args_of<EPI>(a, blocks)); break;
-    case 4: proj_kernel<RT, 4, EPI, W, 0><<<grid_of<EPI>(a, blocks), 64 * W, 0, st>>>(args_of<EPI>(a, blocks)); break;
-    case 8: proj_kernel<RT, 8, EPI, W, 0><<<grid_of<EPI>(a, blocks), 64 * W, 0, st>>>(args_of<EPI>(a, blocks)); break;
-    default: proj_kernel<RT, 16, EPI, W, 0><<<grid_of<EPI>(a, blocks), 64 * W, 0, st>>>(args_of<EPI>(a, blocks)); break;
+    case 0: proj_kernel<RT, 0, EPI, W, 0><<<grid_of<EPI>(a, blocks, 64 * W), 64 * W, 0, st>>>(args_of<EPI>(a, blocks)); break;
+    case 1: proj_kernel<RT, 1, EPI, W, 0><<<grid_of<EPI>(a, blocks, 64 * W), 64 * W, 0, st>>>(args_of<EPI>(a, blocks)); break;
+    case 4: proj_kernel<RT, 4, EPI, W, 0><<<grid_of<EPI>(a, blocks, 64 * W), 64 * W, 0, st>>>(args_of<EPI>(a, blocks)); break;
+    case 8: proj_kernel<RT, 8, EPI, W, 0><<<grid_of<EPI>(a, blocks, 64 * W), 64 * W, 0, st>>>(args_of<EPI>(a, blocks)); break;
+    default: proj_kernel<RT, 16, EPI, W, 0><<<grid_of<EPI>(a, blocks, 64 * W), 64 * W, 0, st>>>(args_of<EPI>(a, blocks)); break;
     }
     return hipGetLastError();
 }
@@ -1471,10 +1474,10 @@ static void launch_p12_c(const ProjArgs& a, uint32_t blocks, hipStream_t st) {
     const uint32_t spw = (a.steps + W - 1) / W;
     // the smallest variant that holds the steps (registers decide how many
     // 16-wavefront blocks a compute unit holds)
-    if (spw <= 2) proj_p12_kernel<RT, EPI, W, 2, CORR><<<grid_of<EPI>(a, blocks), 64 * W, 0, st>>>(args_of<EPI>(a, blocks));
-    else if (spw <= 4) proj_p12_kernel<RT, EPI, W, 4, CORR><<<grid_of<EPI>(a, blocks), 64 * W, 0, st>>>(args_of<EPI>(a, blocks));
-    else if (spw <= 6) proj_p12_kernel<RT, EPI, W, 6, CORR><<<grid_of<EPI>(a, blocks), 64 * W, 0, st>>>(args_of<EPI>(a, blocks));
-    else proj_p12_kernel<RT, EPI, W, 8, CORR><<<grid_of<EPI>(a, blocks), 64 * W, 0, st>>>(args_of<EPI>(a, blocks));
+    if (spw <= 2) proj_p12_kernel<RT, EPI, W, 2, CORR><<<grid_of<EPI>(a, blocks, 64 * W), 64 * W, 0, st>>>(args_of<EPI>(a, blocks));
+    else if (spw <= 4) proj_p12_kernel<RT, EPI, W, 4, CORR><<<grid_of<EPI>(a, blocks, 64 * W), 64 * W, 0, st>>>(args_of<EPI>(a, blocks));
+    else if (spw <= 6) proj_p12_kernel<RT, EPI, W, 6, CORR><<<grid_of<EPI>(a, blocks, 64 * W), 64 * W, 0, st>>>(args_of<EPI>(a, blocks));
+    else proj_p12_kernel<RT, EPI, W, 8, CORR><<<grid_of<EPI>(a, blocks, 64 * W), 64 * W, 0, st>>>(args_of<EPI>(a, blocks));
 }
 template <int RT, int EPI, int W>
 static hipError_t launch_p12_w(const ProjArgs& a, uint32_t blocks, hipStream_t st) {
@@ -1533,7 +1536,7 @@ template <int NM, int KS, int QM, int EPI>
 static void launch_mfma_k(const ProjArgs& a, uint32_t parts, hipStream_t st) {
     constexpr int PD0 = NM == 2 ? LLM_MF_PD2 : LLM_MF_PD1;
     constexpr int PD = PD0 < QM ? PD0 : QM;
-    proj_mfma_kernel<NM, KS, QM, PD, EPI><<<grid_of<EPI>(a, a.nc * parts), 64 * KS, 0, st>>>(
+    proj_mfma_kernel<NM, KS, QM, PD, EPI><<<grid_of<EPI>(a, a.nc * parts, 64 * KS), 64 * KS, 0, st>>>(
         args_of<EPI>(a, a.nc * parts), parts);
 }
 
@@ -1584,7 +1587,7 @@ static void launch_mfma12_k(const ProjArgs& a, uint32_t parts, hipStream_t st) {
     // normalising on load holds the gammas too: one step in flight
     constexpr int PD0 = NM == 2 ? LLM_MF12_PD2 : EPI == EPI_STORE_NORM_IN ? 1 : LLM_MF12_PD1;
     constexpr int PD = PD0 < SM ? PD0 : SM;
-    proj_mfma12_kernel<NM, KS, SM, PD, EPI><<<grid_of<EPI>(a, a.nc * parts), 64 * KS, 0, st>>>(
+    proj_mfma12_kernel<NM, KS, SM, PD, EPI><<<grid_of<EPI>(a, a.nc * parts, 64 * KS), 64 * KS, 0, st>>>(
         args_of<EPI>(a, a.nc * parts), parts);
 }
 

@@ -1960,6 +1960,10 @@ int group_rows(uint32_t T, const llm_adapter_t* adapters, uint32_t count,
         }
         grp.row[grp.rows++] = (uint8_t)r;
     }
+    for (uint32_t g = 0, at = 0; g < 8; g++) {
+        a.start[g] = g < a.groups ? at : ~0u;
+        if (g < a.groups) at += a.g[g].rank;
+    }
     return 0;
 }
 
