@@ -38,7 +38,8 @@ struct SharedAttnArgs {
 };
 // Fills the derived sizes (whole .. own_jobs).
 void shared_attention_shape(SharedAttnArgs& a);
-// Bytes of the scratch, and its parts laid out from `base`.
+// Bytes of the scratch (0: few tiles, none used), and its parts laid out from
+// `base`.
 size_t shared_attention_bytes(const SharedAttnArgs& a);
 void shared_attention_scratch(SharedAttnArgs& a, uint8_t* base);
 hipError_t launch_shared_attention(const SharedAttnArgs& a, hipStream_t st);

@@ -20,7 +20,8 @@
 // heads of a KV group of several sequences side by side), so its K / V pass
 // through the chip once, not once per sequence; a sequence's own tiles are
 // jobs of its own, the first of them beginning with the prefix's last
-// positions where the prefix ends inside a tile.
+// positions where the prefix ends inside a tile.  Up to kSmallTiles tiles, where
+// the launches are what takes the time, one launch does all of it.
 #include "shared_attention.h"
 
 #include "attn_common.h"
@@ -162,14 +163,149 @@ __device__ __noinline__ int32_t defined_score(const int16_t* q, const int16_t* k
     return fx_sat16(fx_rnd(t, 8));
 }
 
+// 16 positions of a tile as operand planes (lane: position lane % 16), their
+// bias 128 sum k' as the products' results lie, whether a value saturates, and
+// whether a lane's part of a bank is all -2048, without which no bank passes
+// 2^31 - 1 (32 products of -32768 and -2048).
+template <int KC>
+struct KeyPlanes {
+    v4i a[KC], b[KC], bias;
+    bool far, low;
+};
+// From raw rows, bank-paired where `paged` (per lane).
+template <int KC, bool ANY>
+__device__ __forceinline__ void key_planes(const v4u (*raw)[2], bool paged, KeyPlanes<KC>& k) {
+    const v4i ones = {0x01010101, 0x01010101, 0x01010101, 0x01010101};
+    uint32_t even = 0x80008000u, odd = 0x80008000u;
+    v4i sa = {0, 0, 0, 0}, sb = sa;
+#pragma unroll
+    for (int kc = 0; kc < KC; kc++) {
+        v4u x = raw[kc][0], y = raw[kc][1];
+        if (!ANY || paged) x = unpair8(x), y = unpair8(y);
+        planes16(x, y, k.a[kc], k.b[kc], even, odd);
+        sa = mfma16(k.a[kc], ones, sa);
+        sb = mfma16(k.b[kc], ones, sb);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) k.bias[i] = 128 * (256 * sa[i] + sb[i]);
+    k.far = __any(sat_mask(max_halves(even, odd)) != 0);
+    constexpr uint32_t kLow = 0xf800f800u;
+    const uint32_t le = even ^ kLow, lo = odd ^ kLow;
+    k.low = KC == 2 && __any((le & 0xffffu) == 0 || (le >> 16) == 0 || (lo & 0xffffu) == 0 ||
+                             (lo >> 16) == 0);
+}
+// The raw values of a lane's K row (0 where there is none) or query.
+template <int KC>
+__device__ __forceinline__ void row_load(const int16_t* row, uint32_t g, uint32_t d,
+                                         v4u (*raw)[2]) {
+#pragma unroll
+    for (int kc = 0; kc < KC; kc++) {
+        const uint32_t e = 64 * kc + 16 * g;
+        raw[kc][0] = raw[kc][1] = v4u{0, 0, 0, 0};
+        if (e < d && row) {
+            raw[kc][0] = *(const v4u*)(row + e);
+            raw[kc][1] = *(const v4u*)(row + e + 8);
+        }
+    }
+}
+// Operand planes in LDS, [KC][2][1024]: c and d of queries, or their c(q).
+template <int KC>
+__device__ __forceinline__ void query_planes(const v4u (*raw)[2], uint32_t lane,
+                                             int8_t (*o)[2][1024]) {
+#pragma unroll
+    for (int kc = 0; kc < KC; kc++) {
+        const v4u u = raw[kc][0], v = raw[kc][1];
+        *(v4i*)&o[kc][0][16 * lane] = v4i{(int32_t)plane_c(u.x, u.y), (int32_t)plane_c(u.z, u.w),
+                                          (int32_t)plane_c(v.x, v.y), (int32_t)plane_c(v.z, v.w)};
+        *(v4i*)&o[kc][1][16 * lane] = v4i{(int32_t)plane_d(u.x, u.y), (int32_t)plane_d(u.z, u.w),
+                                          (int32_t)plane_d(v.x, v.y), (int32_t)plane_d(v.z, v.w)};
+    }
+}
+template <int KC>
+__device__ __forceinline__ void query_corr(const v4u (*raw)[2], uint32_t lane,
+                                           int8_t (*o)[2][1024]) {
+#pragma unroll
+    for (int kc = 0; kc < KC; kc++) {
+        v4i h, l;
+        corr_planes16(raw[kc][0], raw[kc][1], h, l);
+        *(v4i*)&o[kc][0][16 * lane] = h;
+        *(v4i*)&o[kc][1][16 * lane] = l;
+    }
+}
+// Scores of a piece's rows (lane: row lane % 16, query row rho) at positions
+// 16 w + 4 g + s of the job's tile, as packed words; positions that do not
+// count have the lowest.
+template <int KC, bool OWN>
+__device__ __forceinline__ v2u piece_scores(const SharedAttnArgs& a, const Job& b,
+                                            const KeyPlanes<KC>& k, uint32_t w, uint32_t lane,
+                                            uint32_t rho, const int8_t (*qp)[2][1024],
+                                            const int8_t (*corr)[2][1024]) {
+    const uint32_t g = lane >> 4;
+    const v4i zero = {0, 0, 0, 0};
+    v4i ac = zero, x = zero, bd = k.bias;
+#pragma unroll
+    for (int kc = 0; kc < KC; kc++) {
+        const v4i qc = *(const v4i*)&qp[kc][0][16 * lane];
+        const v4i qd = *(const v4i*)&qp[kc][1][16 * lane];
+        ac = mfma16(k.a[kc], qc, ac);
+        x = mfma16(k.a[kc], qd, x);
+        bd = mfma16(k.b[kc], qd, bd);
+        x = mfma16(k.b[kc], qc, x);
+    }
+    if (k.far) {
+#pragma unroll
+        for (int kc = 0; kc < KC; kc++) {
+            const v4i mk = mask2048(k.a[kc], k.b[kc]);
+            x = mfma16(mk, *(const v4i*)&corr[kc][0][16 * lane], x);
+            bd = mfma16(mk, *(const v4i*)&corr[kc][1][16 * lane], bd);
+        }
+    }
+    int32_t sc[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        // sum = 256 t + lo; the two roundings of sum * scale are
+        // floor((sum qk + 2^7 + 2^15) / 2^16) in one, and a t past 2^23 (a sum
+        // past 32 bits) saturates the score
+        const int32_t t = (ac[i] << 8) + x[i] + (bd[i] >> 8);
+        const int32_t lw = __mul24(bd[i] & 255, a.qk_scale) + 32896;
+        sc[i] = (__mul24(med3(t, -(1 << 23), (1 << 23) - 1), a.qk_scale) + (lw >> 8)) >> 8;
+    }
+    if (k.low) {
+        const int16_t* qr = a.q + q_at(a, b.h, rho);
+#pragma unroll 1
+        for (int i = 0; i < 4; i++) {
+            bool paged;
+            const int16_t* kr = k_row(a, b, b.base + 16 * w + 4 * g + i, paged);
+            if (!OWN || kr) {
+                const int32_t v = defined_score(qr, kr, paged, a.head_dim, a.qk_scale);
+                sc[0] = i == 0 ? v : sc[0];
+                sc[1] = i == 1 ? v : sc[1];
+                sc[2] = i == 2 ? v : sc[2];
+                sc[3] = i == 3 ? v : sc[3];
+            }
+        }
+    }
+    if (OWN) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (16 * w + 4 * g + i >= b.valid) sc[i] = INT16_MIN;
+    }
+    return v2u{sat_pack(sc[0], sc[1]), sat_pack(sc[2], sc[3])};
+}
+// The largest of a row's scores over the lanes that hold it.
+__device__ __forceinline__ int32_t row_max(v2u s) {
+    const uint32_t m = max_halves(s.x, s.y);
+    return quad_max(max((int32_t)(int16_t)(m & 0xffffu), (int32_t)m >> 16));
+}
+
 // Scores of the job's rows: wavefront w the tile's positions 16 w .. + 15, so
 // that each K value is loaded and converted once per workgroup, and the byte
 // planes of piece w's queries for all of them.  KC: 64-element chunks of a
 // head.
 template <int KC>
 struct ScoreSmem {
-    int8_t q[kJobPieces][KC][2][1024];  // c, d
-    int8_t corr[kJobPieces][KC][2][1024];  // c(q), where a key value saturates
+    int8_t q[kJobPieces][KC][2][1024];
+    int8_t corr[kJobPieces][KC][2][1024];  // where a key value saturates
     int32_t max[kJobRows][4];
     uint32_t far;
 };
@@ -179,84 +315,21 @@ __device__ __forceinline__ void score_job(const SharedAttnArgs& a, const Job& b,
     const uint32_t lane = threadIdx.x & 63, q = lane & 15, g = lane >> 4, d = a.head_dim;
     const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t nrows = b.end - b.rho;
-    const v4i zero = {0, 0, 0, 0};
-    const v4u none = {0, 0, 0, 0};
-    bool in_page;
-    const int16_t* row = k_row(a, b, b.base + 16 * w + q, in_page);
-    v4u raw[KC][2], qx[KC], qy[KC];
-#pragma unroll
-    for (int kc = 0; kc < KC; kc++) {
-        const uint32_t e = 64 * kc + 16 * g;
-        raw[kc][0] = raw[kc][1] = none;
-        if (e < d && (!OWN || row)) {
-            raw[kc][0] = *(const v4u*)(row + e);
-            raw[kc][1] = *(const v4u*)(row + e + 8);
-        }
-    }
+    bool paged;
+    v4u kraw[KC][2], qraw[KC][2];
+    row_load<KC>(k_row(a, b, b.base + 16 * w + q, paged), g, d, kraw);
     const bool piece = 16 * w < nrows;  // the wavefront has one
-    if (piece) {
-        // rows past the last repeat it
-        const int16_t* qr = a.q + q_at(a, b.h, b.rho + min(16 * w + q, nrows - 1));
-#pragma unroll
-        for (int kc = 0; kc < KC; kc++) {
-            const uint32_t e = 64 * kc + 16 * g;
-            qx[kc] = qy[kc] = none;
-            if (e < d) {
-                qx[kc] = *(const v4u*)(qr + e);
-                qy[kc] = *(const v4u*)(qr + e + 8);
-            }
-        }
-    }
+    if (piece)  // rows past the last repeat it
+        row_load<KC>(a.q + q_at(a, b.h, b.rho + min(16 * w + q, nrows - 1)), g, d, qraw);
     if (threadIdx.x == 0) sm.far = 0;
-    v4i ka[KC], kb[KC], bias;
-    uint32_t even = 0x80008000u, odd = 0x80008000u;
-    {
-        const v4i ones = {0x01010101, 0x01010101, 0x01010101, 0x01010101};
-        v4i sa = zero, sb = zero;
-#pragma unroll
-        for (int kc = 0; kc < KC; kc++) {
-            v4u x = raw[kc][0], y = raw[kc][1];
-            if (!OWN || in_page) x = unpair8(x), y = unpair8(y);
-            planes16(x, y, ka[kc], kb[kc], even, odd);
-            sa = mfma16(ka[kc], ones, sa);
-            sb = mfma16(kb[kc], ones, sb);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; i++) bias[i] = 128 * (256 * sa[i] + sb[i]);
-    }
-    if (piece) {
-#pragma unroll
-        for (int kc = 0; kc < KC; kc++) {
-            const v4u u = qx[kc], v = qy[kc];
-            *(v4i*)&sm.q[w][kc][0][16 * lane] =
-                v4i{(int32_t)plane_c(u.x, u.y), (int32_t)plane_c(u.z, u.w),
-                    (int32_t)plane_c(v.x, v.y), (int32_t)plane_c(v.z, v.w)};
-            *(v4i*)&sm.q[w][kc][1][16 * lane] =
-                v4i{(int32_t)plane_d(u.x, u.y), (int32_t)plane_d(u.z, u.w),
-                    (int32_t)plane_d(v.x, v.y), (int32_t)plane_d(v.z, v.w)};
-        }
-    }
-    // a key value saturates; a lane's part of a bank is all -2048, without
-    // which no bank passes 2^31 - 1 (32 products of -32768 and -2048)
-    const bool far = __any(sat_mask(max_halves(even, odd)) != 0);
-    constexpr uint32_t kLow = 0xf800f800u;
-    const uint32_t le = even ^ kLow, lo = odd ^ kLow;
-    const bool low = KC == 2 && __any((le & 0xffffu) == 0 || (le >> 16) == 0 ||
-                                      (lo & 0xffffu) == 0 || (lo >> 16) == 0);
+    KeyPlanes<KC> k;
+    key_planes<KC, OWN>(kraw, paged, k);
+    if (piece) query_planes<KC>(qraw, lane, sm.q[w]);
     __syncthreads();
-    if (far) sm.far = 1;
+    if (k.far) sm.far = 1;
     __syncthreads();
-    const bool kf = sm.far != 0;
-    if (kf) {
-        if (piece) {
-#pragma unroll
-            for (int kc = 0; kc < KC; kc++) {
-                v4i qh, ql;
-                corr_planes16(qx[kc], qy[kc], qh, ql);
-                *(v4i*)&sm.corr[w][kc][0][16 * lane] = qh;
-                *(v4i*)&sm.corr[w][kc][1][16 * lane] = ql;
-            }
-        }
+    if (sm.far != 0) {
+        if (piece) query_corr<KC>(qraw, lane, sm.corr[w]);
         __syncthreads();
     }
     int16_t* out = a.scores +
@@ -264,59 +337,11 @@ __device__ __forceinline__ void score_job(const SharedAttnArgs& a, const Job& b,
 #pragma unroll 1
     for (uint32_t r0 = 0; r0 < nrows; r0 += 16) {
         const uint32_t p = r0 / 16;
-        v4i ac = zero, x = zero, bd = bias;
-#pragma unroll
-        for (int kc = 0; kc < KC; kc++) {
-            const v4i qc = *(const v4i*)&sm.q[p][kc][0][16 * lane];
-            const v4i qd = *(const v4i*)&sm.q[p][kc][1][16 * lane];
-            ac = mfma16(ka[kc], qc, ac);
-            x = mfma16(ka[kc], qd, x);
-            bd = mfma16(kb[kc], qd, bd);
-            x = mfma16(kb[kc], qc, x);
-        }
-        if (kf) {
-#pragma unroll
-            for (int kc = 0; kc < KC; kc++) {
-                const v4i mk = mask2048(ka[kc], kb[kc]);
-                x = mfma16(mk, *(const v4i*)&sm.corr[p][kc][0][16 * lane], x);
-                bd = mfma16(mk, *(const v4i*)&sm.corr[p][kc][1][16 * lane], bd);
-            }
-        }
-        int32_t sc[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            // sum = 256 t + lo; the two roundings of sum * scale are
-            // floor((sum qk + 2^7 + 2^15) / 2^16) in one, and a t past 2^23 (a
-            // sum past 32 bits) saturates the score
-            const int32_t t = (ac[i] << 8) + x[i] + (bd[i] >> 8);
-            const int32_t lw = __mul24(bd[i] & 255, a.qk_scale) + 32896;
-            sc[i] = (__mul24(med3(t, -(1 << 23), (1 << 23) - 1), a.qk_scale) + (lw >> 8)) >> 8;
-        }
-        if (low) {
-            const int16_t* qr = a.q + q_at(a, b.h, b.rho + min(r0 + q, nrows - 1));
-#pragma unroll 1
-            for (int i = 0; i < 4; i++) {
-                bool paged;
-                const int16_t* kr = k_row(a, b, b.base + 16 * w + 4 * g + i, paged);
-                if (!OWN || kr) {
-                    const int32_t v = defined_score(qr, kr, paged, d, a.qk_scale);
-                    sc[0] = i == 0 ? v : sc[0];
-                    sc[1] = i == 1 ? v : sc[1];
-                    sc[2] = i == 2 ? v : sc[2];
-                    sc[3] = i == 3 ? v : sc[3];
-                }
-            }
-        }
-        if (OWN) {
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (16 * w + 4 * g + i >= b.valid) sc[i] = INT16_MIN;
-        }
-        const uint32_t s0 = sat_pack(sc[0], sc[1]), s1 = sat_pack(sc[2], sc[3]);
-        const uint32_t m = max_halves(s0, s1);
-        const int32_t mx = quad_max(max((int32_t)(int16_t)(m & 0xffffu), (int32_t)m >> 16));
+        const v2u s = piece_scores<KC, OWN>(a, b, k, w, lane, b.rho + min(r0 + q, nrows - 1),
+                                            sm.q[p], sm.corr[p]);
+        const int32_t mx = row_max(s);
         if (r0 + q < nrows) {
-            *(v2u*)(out + (r0 + q) * TILE) = v2u{s0, s1};
+            *(v2u*)(out + (r0 + q) * TILE) = s;
             if (g == 0) sm.max[r0 + q][w] = mx;
         }
     }
@@ -382,6 +407,77 @@ __device__ __forceinline__ void own_values(const SharedAttnArgs& a, const Job& b
                 __builtin_amdgcn_perm(y[u], x[u], 0x07060302u);
         }
     }
+}
+
+// Probabilities of a lane's 16 positions (natural order) from their scores and
+// the running maximum, as packed words, and their sum; MASK: positions from
+// `valid` on, counted from the lane's first, have none.
+template <bool MASK>
+__device__ __forceinline__ int32_t row_probs(v4u s0, v4u s1, int32_t top, int32_t valid,
+                                             const int16_t* e14, uint32_t* pw) {
+    const uint32_t tops = pack16(top, top);
+    const s16x2 floor2 = {-2048, -2048};
+    int32_t sum = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        // sat16(s - top), not below -2048
+        const uint32_t s = i < 4 ? s0[i] : s1[i - 4];
+        const s16x2 x = __builtin_elementwise_max(
+            __builtin_elementwise_sub_sat(halves(s), halves(tops)), floor2);
+        int32_t p0 = e14[x.x + 2048], p1 = e14[x.y + 2048];
+        if (MASK) {
+            p0 = 2 * i < valid ? p0 : 0;
+            p1 = 2 * i + 1 < valid ? p1 : 0;
+        }
+        pw[i] = pack16(p0, p1);
+        sum = dot2(pw[i], 0x00010001u, sum);
+    }
+    return sum;
+}
+// Their operand planes in LDS, [4][1024]: p, and (corr) c(p).
+__device__ __forceinline__ void prob_planes(const uint32_t* pw, uint32_t lane,
+                                            int8_t (*o)[1024]) {
+    v4i pc, pd;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        // p + 128 <= 16512: no carry between the halves
+        pc[i] = (int32_t)plane_c(pw[2 * i] + 0x00800080u, pw[2 * i + 1] + 0x00800080u);
+        pd[i] = (int32_t)low_plane(pw[2 * i], pw[2 * i + 1]);
+    }
+    *(v4i*)&o[0][16 * lane] = pc;
+    *(v4i*)&o[1][16 * lane] = pd;
+}
+__device__ __forceinline__ void prob_corr(const uint32_t* pw, uint32_t lane, int8_t (*o)[1024]) {
+    v4i ph, pq;
+    corr_planes16(v4u{pw[0], pw[1], pw[2], pw[3]}, v4u{pw[4], pw[5], pw[6], pw[7]}, ph, pq);
+    *(v4i*)&o[2][16 * lane] = ph;
+    *(v4i*)&o[3][16 * lane] = pq;
+}
+// Tile values of a strip (lane: row lane % 16, elements 4 (lane / 16) + s) as
+// packed words.
+__device__ __forceinline__ v2u strip_values(v4i va, v4i vb, bool far, uint32_t lane,
+                                            const int8_t (*pl)[1024]) {
+    const v4i zero = {0, 0, 0, 0}, half = {8224, 8224, 8224, 8224};
+    const v4i pc = *(const v4i*)&pl[0][16 * lane], pd = *(const v4i*)&pl[1][16 * lane];
+    v4i ac = mfma16(va, pc, zero);
+    v4i x = mfma16(va, pd, zero);
+    v4i bd = mfma16(vb, pd, half);
+    x = mfma16(vb, pc, x);
+    if (far) {
+        const v4i mk = mask2048(va, vb);
+        x = mfma16(mk, *(const v4i*)&pl[2][16 * lane], x);
+        bd = mfma16(mk, *(const v4i*)&pl[3][16 * lane], bd);
+    }
+    int32_t tv[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        // sums in [-2^31, 2^31 - 2^16] (64 products of at most 2^14 and -2048,
+        // or 2048 with its correction of -1024): exact in 32 bits, and so with
+        // 8224 added; rnd(rnd(tot, 6), 8) = floor((tot + 2^5 + 2^13) / 2^14)
+        const uint32_t tot = ((((uint32_t)ac[i] << 8) + (uint32_t)x[i]) << 8) + (uint32_t)bd[i];
+        tv[i] = (int32_t)tot >> 14;
+    }
+    return v2u{sat_pack(tv[0], tv[1]), sat_pack(tv[2], tv[3])};
 }
 
 struct ValueSmem {
@@ -466,33 +562,9 @@ __device__ __forceinline__ void value_job(const SharedAttnArgs& a, const Job& b,
 #pragma unroll
         for (int u = 0; u < 4; u++) before = max(before, (int32_t)sm.hist[u][skip + r]);
         const int32_t top = max(before, tmj);
-        const uint32_t tops = pack16(top, top);
-        const s16x2 floor2 = {-2048, -2048};
-        int32_t sum = 0;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            // sat16(s - top), not below -2048
-            const uint32_t s = i < 4 ? s0[i] : s1[i - 4];
-            const s16x2 x = __builtin_elementwise_max(
-                __builtin_elementwise_sub_sat(halves(s), halves(tops)), floor2);
-            int32_t p0 = sm.e14[x.x + 2048], p1 = sm.e14[x.y + 2048];
-            if (OWN) {
-                p0 = 16 * g + 2 * i < b.valid ? p0 : 0;
-                p1 = 16 * g + 2 * i + 1 < b.valid ? p1 : 0;
-            }
-            pw[i] = pack16(p0, p1);
-            sum = dot2(pw[i], 0x00010001u, sum);
-        }
-        v4i pc, pd;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            // p + 128 <= 16512: no carry between the halves
-            pc[i] = (int32_t)plane_c(pw[2 * i] + 0x00800080u, pw[2 * i + 1] + 0x00800080u);
-            pd[i] = (int32_t)low_plane(pw[2 * i], pw[2 * i + 1]);
-        }
-        *(v4i*)&sm.planes[w][0][16 * lane] = pc;
-        *(v4i*)&sm.planes[w][1][16 * lane] = pd;
-        sum = quad_sum(sum);
+        const int32_t sum = quad_sum(row_probs<OWN>(
+            s0, s1, top, (int32_t)b.valid - 16 * (int32_t)g, sm.e14, pw));
+        prob_planes(pw, lane, sm.planes[w]);
         if (g == 0 && 16 * w + q < nrows) {
             a.tsum[trow + r] = sum << 2;
             a.old[trow + r] = (int32_t)sm.e14[max(before - top, -2048) + 2048] << 2;
@@ -514,53 +586,19 @@ __device__ __forceinline__ void value_job(const SharedAttnArgs& a, const Job& b,
     __syncthreads();
     const bool vf = sm.far != 0;
     if (vf) {
-        if (piece) {
-            v4i ph, pq;
-            corr_planes16(v4u{pw[0], pw[1], pw[2], pw[3]}, v4u{pw[4], pw[5], pw[6], pw[7]}, ph, pq);
-            *(v4i*)&sm.planes[w][2][16 * lane] = ph;
-            *(v4i*)&sm.planes[w][3][16 * lane] = pq;
-        }
+        if (piece) prob_corr(pw, lane, sm.planes[w]);
         __syncthreads();
     }
     // ---- values ----
-    const v4i zero = {0, 0, 0, 0}, half = {8224, 8224, 8224, 8224};
     int16_t* out = a.tval + trow * d + 4 * g;
 #pragma unroll 1
     for (uint32_t r0 = 0; r0 < nrows; r0 += 16) {
-        const int8_t(*pl)[1024] = sm.planes[r0 / 16];
-        const v4i pc = *(const v4i*)&pl[0][lane * 16], pd = *(const v4i*)&pl[1][lane * 16];
-        v4i ph = zero, pq = zero;
-        if (vf) {
-            ph = *(const v4i*)&pl[2][lane * 16];
-            pq = *(const v4i*)&pl[3][lane * 16];
-        }
         const bool real = r0 + q < nrows;
 #pragma unroll
         for (int es = 0; es < ES; es++) {
-            v4i ac = mfma16(va[es], pc, zero);
-            v4i x = mfma16(va[es], pd, zero);
-            v4i bd = mfma16(vb[es], pd, half);
-            x = mfma16(vb[es], pc, x);
-            if (vf) {
-                const v4i mk = mask2048(va[es], vb[es]);
-                x = mfma16(mk, ph, x);
-                bd = mfma16(mk, pq, bd);
-            }
-            int32_t tv[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                // sums in [-2^31, 2^31 - 2^16] (64 products of at most 2^14
-                // and -2048, or 2048 with its correction of -1024): exact in
-                // 32 bits, and so with 8224 added; rnd(rnd(tot, 6), 8) =
-                // floor((tot + 2^5 + 2^13) / 2^14)
-                const uint32_t tot = ((((uint32_t)ac[i] << 8) + (uint32_t)x[i]) << 8) +
-                                     (uint32_t)bd[i];
-                tv[i] = (int32_t)tot >> 14;
-            }
+            const v2u tv = strip_values(va[es], vb[es], vf, lane, sm.planes[r0 / 16]);
             const uint32_t st = w + 4 * es;
-            if (real && st < ne)
-                *(v2u*)(out + (r0 + q) * d + 16 * st) =
-                    v2u{sat_pack(tv[0], tv[1]), sat_pack(tv[2], tv[3])};
+            if (real && st < ne) *(v2u*)(out + (r0 + q) * d + 16 * st) = tv;
         }
     }
 }
@@ -696,6 +734,150 @@ __global__ __launch_bounds__(256) void shared_join_kernel(SharedAttnArgs a) {
     }
 }
 
+// Few tiles: the whole attention of one sequence and KV head by one workgroup:
+// scores (wavefront w positions 16 w .. + 15 of each tile), probabilities
+// (wavefront w tile w's), values and the chain (wavefront w strips w, w + 4,
+// the accumulators in registers).  One launch in place of three, but the shared
+// tiles' keys and values are converted for each sequence, and a workgroup takes
+// its tiles one after another.  Back to back, this and the three launches: head
+// dimension 64, 2 KV heads, 8 sequences: 2 tiles 7.9 and 12.5 us, 4 tiles 10.2
+// and 12.5, 8 tiles 16.1 and 12.6; dimension 128: 2 tiles 10.9 and 14.6, 4
+// tiles 14.8 and 15.4, 8 tiles 24.1 and 15.6.  8 KV heads, 64 sequences, 4
+// tiles: 20.4 and 39.0.
+constexpr uint32_t kSmallTiles = 4;
+template <int KC>
+struct SmallSmem {
+    int8_t q[KC][2][1024], corr[KC][2][1024];
+    int16_t e14[2056];
+    int16_t s[kSmallTiles][16][72];      // scores; rows 144 bytes apart
+    int32_t max[kSmallTiles][16][4];
+    int32_t old[kSmallTiles][16], sum[kSmallTiles][16];
+    int8_t planes[kSmallTiles][4][1024];
+    int16_t vt[128 * kOwnRow];
+};
+template <int KC>
+__global__ __launch_bounds__(256) void shared_small_kernel(SharedAttnArgs a) {
+    constexpr int ES = KC;
+    __shared__ __attribute__((aligned(16))) SmallSmem<KC> sm;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, q = lane & 15, g = lane >> 4;
+    const uint32_t w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t d = a.head_dim, ne = d / 16;
+    Job b;
+    b.h = blockIdx.x % a.kv_heads;
+    b.seq = blockIdx.x / a.kv_heads;
+    b.rho = b.seq * a.group;
+    b.end = b.rho + a.group;
+    b.own = true;
+    const uint32_t rho = min(b.rho + q, b.end - 1);  // rows past the last repeat it
+    if (w == 0) {
+        v4u qraw[KC][2];
+        row_load<KC>(a.q + q_at(a, b.h, rho), g, d, qraw);
+        query_planes<KC>(qraw, lane, sm.q);
+        query_corr<KC>(qraw, lane, sm.corr);
+    }
+    *(v4u*)(sm.e14 + 8 * tid) = *(const v4u*)(a.exp14 + 8 * tid);
+    if (tid == 0) *(v4u*)(sm.e14 + 2048) = *(const v4u*)(a.exp14 + 2048);
+    const uint32_t n = a.prefix + length_of(a, b.seq), nt = (n + 63) / 64;
+    int32_t before = INT16_MIN, total = 0, acc[ES][4];
+#pragma unroll
+    for (int es = 0; es < ES; es++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[es][i] = 0;
+    if (nt > 0) {  // the whole workgroup alike
+        auto tile = [&](uint32_t t) {
+            b.j = t;
+            b.base = 64 * t;
+            b.valid = min(n - b.base, 64u);
+        };
+        v4u kraw[kSmallTiles][KC][2];
+        bool paged[kSmallTiles];
+#pragma unroll
+        for (uint32_t i = 0; i < kSmallTiles; i++) {
+            tile(min(i, nt - 1));
+            row_load<KC>(k_row(a, b, b.base + 16 * w + q, paged[i]), g, d, kraw[i]);
+        }
+        __syncthreads();  // the queries' planes
+#pragma unroll
+        for (uint32_t i = 0; i < kSmallTiles; i++) {
+            if (i >= nt) break;
+            tile(i);
+            KeyPlanes<KC> k;
+            key_planes<KC, true>(kraw[i], paged[i], k);
+            const v2u s = piece_scores<KC, true>(a, b, k, w, lane, rho, sm.q, sm.corr);
+            *(v2u*)&sm.s[i][q][16 * w + 4 * g] = s;
+            const int32_t mx = row_max(s);
+            if (g == 0) sm.max[i][q][w] = mx;
+        }
+        __syncthreads();
+        // ---- probabilities ----
+#pragma unroll
+        for (uint32_t i = 0; i < kSmallTiles; i++) {
+            if (i >= nt) break;
+            const v4i m = *(const v4i*)sm.max[i][q];
+            const int32_t next = max(before, max(max(m[0], m[1]), max(m[2], m[3])));
+            if (i == w) {
+                tile(i);
+                uint32_t pw[8];
+                const int32_t sum = quad_sum(row_probs<true>(
+                    *(const v4u*)&sm.s[i][q][16 * g], *(const v4u*)&sm.s[i][q][16 * g + 8], next,
+                    (int32_t)b.valid - 16 * (int32_t)g, sm.e14, pw));
+                prob_planes(pw, lane, sm.planes[i]);
+                prob_corr(pw, lane, sm.planes[i]);
+                if (g == 0) {
+                    sm.sum[i][q] = sum << 2;
+                    sm.old[i][q] = (int32_t)sm.e14[max(before - next, -2048) + 2048] << 2;
+                }
+            }
+            before = next;
+        }
+        // ---- values and the chain ----
+#pragma unroll 1
+        for (uint32_t i = 0; i < nt; i++) {
+            tile(i);
+            const bool page = b.base + 64 <= a.prefix;  // all of it in one
+            if (!page) {
+                if (i > 0) __syncthreads();  // what the last tile's strips read
+                own_values(a, b, sm.vt);
+            }
+            if (!page || i == 0) __syncthreads();
+            const int32_t old = sm.old[i][q];
+            total = __builtin_elementwise_add_sat(rnd16_mul(total, old), sm.sum[i][q]);
+            const int16_t* src = a.vcache + ((size_t)b.h * a.pages + b.j) * TILE * d;
+#pragma unroll
+            for (int es = 0; es < ES; es++) {
+                const uint32_t e = 16 * min(w + 4 * es, ne - 1) + q;  // past the last: repeated
+                v4u x, y;
+                if (page) {
+                    x = unpair8(*(const v4u*)(src + e * TILE + 16 * g));
+                    y = unpair8(*(const v4u*)(src + e * TILE + 16 * g + 8));
+                } else {
+                    x = *(const v4u*)(sm.vt + e * kOwnRow + 16 * g);
+                    y = *(const v4u*)(sm.vt + e * kOwnRow + 16 * g + 8);
+                }
+                v4i va, vb;
+                uint32_t even = 0x80008000u, odd = 0x80008000u;
+                planes16(x, y, va, vb, even, odd);
+                const v2u tv = strip_values(va, vb, __any(sat_mask(max_halves(even, odd)) != 0),
+                                            lane, sm.planes[i]);
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+                    acc[es][u] = __builtin_elementwise_add_sat(rnd16_mul(acc[es][u], old),
+                                                               half16(tv, u) << 8);
+            }
+        }
+    }
+    const int32_t inv = fx_inv_sum(total);
+    int16_t* out = a.out + q_at(a, b.h, rho) + 4 * g;
+#pragma unroll
+    for (int es = 0; es < ES; es++) {
+        int32_t y[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) y[i] = rnd16_mul(acc[es][i], inv);
+        if (q < a.group && w + 4 * es < ne)
+            *(v2u*)(out + 16 * (w + 4 * es)) = v2u{sat_pack(y[0], y[1]), sat_pack(y[2], y[3])};
+    }
+}
+
 uint32_t round_to(uint32_t v, uint32_t m) { return (v + m - 1) / m * m; }
 size_t part_bytes(size_t n) { return (n + 255) / 256 * 256; }
 
@@ -715,12 +897,14 @@ void shared_attention_shape(SharedAttnArgs& a) {
 }
 
 size_t shared_attention_bytes(const SharedAttnArgs& a) {
+    if (a.tiles <= kSmallTiles) return 0;
     const size_t rt = (size_t)a.kv_heads * a.tiles * a.rows_pad;
     return part_bytes(rt * 64 * 2) + part_bytes(rt * 2) + 2 * part_bytes(rt * 4) +
            part_bytes(rt * a.head_dim * 2);
 }
 
 void shared_attention_scratch(SharedAttnArgs& a, uint8_t* base) {
+    if (a.tiles <= kSmallTiles) return;
     const size_t rt = (size_t)a.kv_heads * a.tiles * a.rows_pad;
     auto take = [&](size_t bytes) {
         uint8_t* p = base;
@@ -735,21 +919,27 @@ void shared_attention_scratch(SharedAttnArgs& a, uint8_t* base) {
 }
 
 hipError_t launch_shared_attention(const SharedAttnArgs& a, hipStream_t st) {
-    const uint32_t grid = a.shared_jobs + a.own_jobs;
-    if (grid) {
+    if (a.tiles <= kSmallTiles) {
+        const uint32_t grid = a.kv_heads * a.sequences;
         if (a.head_dim <= 64)
-            shared_scores_kernel<1><<<grid, 256, 0, st>>>(a);
+            shared_small_kernel<1><<<grid, 256, 0, st>>>(a);
         else
-            shared_scores_kernel<2><<<grid, 256, 0, st>>>(a);
-        hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
-        if (a.head_dim <= 64)
-            shared_values_kernel<1><<<grid, 256, 0, st>>>(a);
-        else
-            shared_values_kernel<2><<<grid, 256, 0, st>>>(a);
-        e = hipGetLastError();
-        if (e != hipSuccess) return e;
+            shared_small_kernel<2><<<grid, 256, 0, st>>>(a);
+        return hipGetLastError();
     }
+    const uint32_t grid = a.shared_jobs + a.own_jobs;
+    if (a.head_dim <= 64)
+        shared_scores_kernel<1><<<grid, 256, 0, st>>>(a);
+    else
+        shared_scores_kernel<2><<<grid, 256, 0, st>>>(a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    if (a.head_dim <= 64)
+        shared_values_kernel<1><<<grid, 256, 0, st>>>(a);
+    else
+        shared_values_kernel<2><<<grid, 256, 0, st>>>(a);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
     const dim3 rows(a.kv_heads * a.rows, (a.head_dim + 63) / 64);
     shared_join_kernel<<<rows, 256, 0, st>>>(a);
     return hipGetLastError();
