@@ -254,7 +254,9 @@ int llm_op(llm_ctx_t* ctx, uint32_t op, uint32_t layer, uint32_t token_count,
  * [token_count] are host memory, read before the call returns.  in and out
  * are device memory as in llm_op (NULL: the context's ports; in at an 8-byte
  * address; they may overlap).  Returns llm_op's status codes and counters;
- * work is enqueued and not waited for.  The first call allocates. */
+ * work is enqueued and not waited for.  The first call allocates scratch that
+ * is the context's: graphs that hold such calls must not run beside one
+ * another or beside the context's own work. */
 typedef struct {
     const int16_t* a;
     const int16_t* b;
@@ -276,12 +278,14 @@ int llm_op_adapted(llm_ctx_t* ctx, uint32_t op, uint32_t layer, uint32_t token_c
  * then the sequence's own positions, bit for bit; a sequence with no position
  * at all gets zeros.  Rows behind own_len are neither read nor written.
  * 1..64 sequences, prefix_len <= max_seq_len, own_capacity <= 2^20 (0: k_own,
- * v_own and own_len may be NULL); q, out, k_own and v_own start at 16-byte
- * addresses; out may be q.  Work is enqueued and not waited for; own_len is
- * read when it runs.  A call that needs more scratch than any before
- * allocates (per query row and tile of 64 positions 136 + 2 d bytes); the
- * scratch is the context's, so graphs that hold such calls must not run
- * beside one another or beside the context's own work. */
+ * v_own and own_len may be NULL), below 2^24 tiles of 64 positions over all
+ * KV heads (the prefix's once per 64 rows of a KV head, the others per
+ * sequence); q, out, k_own and v_own start at 16-byte addresses; out may be q.
+ * Work is enqueued and not waited for; own_len is read when it runs.  A call
+ * of more than 4 tiles that needs more scratch than any before allocates (per
+ * query row and tile 138 + 2 d bytes); the scratch is the context's, so graphs
+ * that hold such calls must not run beside one another or beside the context's
+ * own work. */
 #define LLM_SHARED_SEQUENCES 64u
 #define LLM_SHARED_OWN_CAPACITY (1u << 20)
 int llm_attention_shared(llm_ctx_t* ctx, uint32_t layer, uint32_t prefix_len,

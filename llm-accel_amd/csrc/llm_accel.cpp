@@ -2047,6 +2047,11 @@ int llm_attention_shared(llm_ctx_t* c, uint32_t layer, uint32_t prefix, uint32_t
     a.head_dim = c->d;
     a.qk_scale = c->qk_scale;
     a.exp14 = c->exp14;
+    // the launches' workgroups, 256 threads each, count their threads in 32 bits
+    const uint64_t own_tiles = ((uint64_t)prefix % 64 + own_capacity + 63) / 64;
+    const uint64_t groups = ((uint64_t)sequences * c->G + 63) / 64;
+    if (c->Hkv * (prefix / 64 * groups + sequences * own_tiles) >= 1u << 24)
+        return fail(LLM_E_ARG, "more than 2^24 tiles of sequences and KV heads");
     llm::shared_attention_shape(a);
     HIP_TRY(hipSetDevice(c->device));
     const size_t need = llm::shared_attention_bytes(a);

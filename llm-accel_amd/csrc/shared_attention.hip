@@ -615,13 +615,13 @@ __global__ __launch_bounds__(256, 4) void shared_values_kernel(SharedAttnArgs a)
 }
 
 // The chain over a row's tiles, one workgroup per row and 64 head elements.  A
-// thread loads 8 of the elements of 8 consecutive tiles (a run), all of them at once, and leaves
-// them and their sums over the run in LDS; a wavefront then walks the runs
-// while the next block's loads are under way.  A run over which the maximum does not
-// rise (old = 1.0 throughout: most, once the first tiles are past) is one
-// addition of its sum, four such runs at a time: exact, because the
-// probabilities' sums are not negative and the elements' 32 values (at most
-// 2^28 together) cannot saturate an accumulator within 2^30.
+// thread loads 8 of the elements of 8 consecutive tiles (a run), all of them
+// at once, and leaves them and their sums over the run in LDS; a wavefront then
+// walks the runs while the next block's loads are under way.  A run over which
+// the maximum does not rise (old = 1.0 throughout: most, once the first tiles
+// are past) is one addition of its sum, four such runs at a time: exact,
+// because the probabilities' sums are not negative and the elements' 32 values
+// (at most 2^28 together) cannot saturate an accumulator within 2^30.
 __global__ __launch_bounds__(256) void shared_join_kernel(SharedAttnArgs a) {
     constexpr uint32_t EC = 8, RUNS = 256 / EC, BLOCK = 8 * RUNS;
     __shared__ __attribute__((aligned(16))) int16_t s_v[BLOCK][8 * EC];

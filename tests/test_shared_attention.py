@@ -251,3 +251,18 @@ def test_refusals():
         acc.attention_shared(*good)
         acc.attention_shared(0, 100, 2, p, None, None, None, 0, p)
         acc.sync()
+
+
+@pytest.mark.gpu
+def test_refuses_more_tiles_than_a_launch_counts():
+    """16 KV heads, 64 sequences of up to 2^20 positions: 2^24 tiles.  The
+    buffers are never reached; 63 sequences of 2^14 positions are fine."""
+    with _accelerator(16, 16, 16, 64) as acc, Hip() as hip:
+        p = hip.alloc(1 << 20)
+        with pytest.raises(llm_accel.AccelError, match="tiles"):
+            acc.attention_shared(0, 0, 64, p, p, p, p, 1 << 20, p)
+        hip.put(np.zeros(64, np.uint32), to=p)  # no sequence has a position
+        out = hip.put(np.full(63 * 16 * 16, 5, np.int16))
+        acc.attention_shared(0, 0, 63, out, p, p, p, 1 << 14, out)
+        acc.sync()
+        assert not hip.get(out, 63 * 16 * 16, np.int16).any()
