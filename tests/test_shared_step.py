@@ -60,7 +60,7 @@ def test_steps_of_requests_that_share_a_prompt(plen):
                   for rank in (8, 20)] for p in range(7)] for la in range(layers)]
     norm16 = lambda s, *sh: np.round(rng.standard_normal(sh) * 256 * s).astype(np.int16)  # noqa: E731,E501
     prefix = norm16(1.0, layers, kv, plen, d), norm16(0.5, layers, kv, plen, d)
-    temperatures = [0.7, 1.0, 0.4]
+    temperatures = [30.0, 64.0, 40.0]  # the synthetic head's scores spread over 100 and more
     # what each request has generated: K / V per layer [n][kv][d], last token
     past = [[(np.zeros((0, kv, d), np.int16),) * 2 for _ in range(layers)] for _ in counts]
     last = rng.integers(0, spec.vocab, len(counts)).tolist()
