@@ -143,11 +143,15 @@ hipError_t launch_io_rows(const int16_t* src, uint32_t ld_src, int16_t* dst, uin
 hipError_t launch_lm_argmax(const int16_t* w, uint32_t steps, uint32_t n,
                             const int16_t* x, uint32_t ldx, uint32_t rows, int L,
                             unsigned long long* keys, hipStream_t st);
-// The same, and every score: scores[r][v] (row stride lds, a multiple of 16).
+// The same, and every score: of 16 tokens, the rows' one after the other (a
+// workgroup's are consecutive: 8 rows of 151,936 x 2,048 in 109.4 us, in rows
+// of all tokens 112.8).
+__host__ __device__ inline size_t score_at(uint32_t v, uint32_t r, uint32_t rows) {
+    return ((size_t)(v >> 4) * rows + r) * 16 + (v & 15);
+}
 hipError_t launch_lm_scores(const int16_t* w, uint32_t steps, uint32_t n,
                             const int16_t* x, uint32_t ldx, uint32_t rows, int L,
-                            unsigned long long* keys, int64_t* scores, uint32_t lds,
-                            hipStream_t st);
+                            unsigned long long* keys, int64_t* scores, hipStream_t st);
 // Blocks of at least kMfMinRows rows run on the matrix cores when the
 // byte-plane layout is present; others on the VALU dot2 kernel.
 #ifndef LLM_MF_MIN_ROWS

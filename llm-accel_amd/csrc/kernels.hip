@@ -1002,8 +1002,7 @@ __global__ __launch_bounds__(64 * KS) void proj_mfma12_kernel(typename ArgsOf<EP
 // at most kLmStageSteps k-steps) and every step reads them from there, so
 // that the loads in the loop are the table's only (the four lanes of a
 // column group read the same 16 bytes: an LDS broadcast).
-// SC: the scores themselves are kept too, scores[r][v] of row stride lds (a
-// multiple of 16).
+// SC: the scores themselves are kept too (score_at).
 constexpr uint32_t kLmStageSteps = 32;
 template <int RT, int L, bool XS = false, bool SC = false>
 __global__ __launch_bounds__(256) void lm_argmax_kernel(const int16_t* __restrict__ w,
@@ -1011,8 +1010,7 @@ __global__ __launch_bounds__(256) void lm_argmax_kernel(const int16_t* __restric
                                                         const int16_t* __restrict__ x,
                                                         uint32_t ldx, uint32_t rows,
                                                         unsigned long long* keys,
-                                                        int64_t* __restrict__ scores,
-                                                        uint32_t lds) {
+                                                        int64_t* __restrict__ scores) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int i = lane >> 4, j = lane & 15;
     const uint32_t nblocks = (n + 3) / 4;
@@ -1073,7 +1071,7 @@ __global__ __launch_bounds__(256) void lm_argmax_kernel(const int16_t* __restric
             acc[r] = row16_sum(acc[r]);
             const unsigned long long k = argmax_key(acc[r], v);
             if (j == 15 && v < n && k > best[r]) best[r] = k;
-            if (SC && j == 15 && v < n && r < (int)rows) scores[(size_t)r * lds + v] = acc[r];
+            if (SC && j == 15 && v < n && r < (int)rows) scores[score_at(v, r, rows)] = acc[r];
         }
     }
     __shared__ unsigned long long wbest[4][4][RT];
@@ -1093,8 +1091,9 @@ __global__ __launch_bounds__(256) void lm_argmax_kernel(const int16_t* __restric
 
 // The same for blocks of 3-8 rows on the matrix cores: the VALU kernel's
 // products grow with the rows (8 rows of the 151,936 x 2,048 table: call
-// 415-421 us against 107-116 for one, whose time is the table's bytes; here
-// 127-135, the kernel 117 of them).  With w = 256 a + b + 128 and x = 256 c + d + 128 (signed bytes),
+// 415-421 us against 107-116 for one, whose time is the table's bytes; here the
+// kernel takes 102, 6.1 TB/s, and 109 where it stores the scores).  With w =
+// 256 a + b + 128 and x = 256 c + d + 128 (signed bytes),
 //   sum w x = 65536 sum ac + 256 (sum ad + sum bc) + sum bd
 //             + 128 sum (256 a + b) + 128 sum x,
 // all sums exact in int32 (hidden <= 3840 here): the MFMA's columns are the
@@ -1102,24 +1101,29 @@ __global__ __launch_bounds__(256) void lm_argmax_kernel(const int16_t* __restric
 // then b, and a product with ones gives sum a and sum b.  The activations
 // wait in LDS in operand order; a lane's table bytes are 8-column pieces
 // (columns 32 q + 8 g of a step), so that each load of a wavefront covers
-// 64 contiguous bytes of 16 rows.  A wavefront walks 16-row groups, or, for
-// tables of few groups (KS), the four wavefronts of a workgroup share one.
+// 64 contiguous bytes of 16 rows.  The four wavefronts of a workgroup share
+// the steps of a 16-row group (KS; where their sums do not fit into LDS a
+// wavefront takes a group), with the loads of AHEAD steps in flight across
+// groups.  Workgroups begin a group at different steps, because in step they
+// meet in the same memory channels: 151,936 and 50,000 rows of 2,048 in 102
+// and 40 us, from step 0 on 106 and 43; a wavefront per group 104 and 45, from
+// step 0 on 125 and 54.
 constexpr uint32_t kLmGroup = 16;
 // Activations of at most 60 KiB (44 with the shared groups' sums) in LDS.
 constexpr uint32_t kLmMfmaSteps = 30, kLmMfmaStepsShared = 22;
-template <bool KS, bool SC = false>
+template <bool KS, bool SC, uint32_t AHEAD>
 __global__ __launch_bounds__(256) void lm_argmax_mfma_kernel(const int16_t* __restrict__ w,
                                                              uint32_t S, uint32_t n,
                                                              const int16_t* __restrict__ x,
                                                              uint32_t ldx, uint32_t rows,
                                                              unsigned long long* keys,
-                                                             int64_t* __restrict__ scores,
-                                                             uint32_t lds) {
+                                                             int64_t* __restrict__ scores) {
     extern __shared__ __attribute__((aligned(16))) int8_t lm_x[];  // [S][2][64][16]
     __shared__ int32_t xsum[8];
     __shared__ unsigned long long wbest[4][16];
-    __shared__ v4i red[KS ? 4 : 1][4][64];
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    __shared__ v4i red[2][KS ? 3 : 1][3][64];
+    const uint32_t tid = threadIdx.x, lane = tid & 63;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t j = lane & 15, g = lane >> 4;
     if (tid < 8) xsum[tid] = 0;
     __syncthreads();
@@ -1144,85 +1148,129 @@ __global__ __launch_bounds__(256) void lm_argmax_mfma_kernel(const int16_t* __re
     __syncthreads();
     const uint32_t ngroups = (n + kLmGroup - 1) / kLmGroup, nblk = (n + 3) / 4;
     const v4i ones = {0x01010101, 0x01010101, 0x01010101, 0x01010101};
-    const uint32_t s0 = KS ? wave * S / 4 : 0, s1 = KS ? (wave + 1) * S / 4 : S;
+    // the wavefront's steps of a group (KS: one that no sum counts where there
+    // are fewer steps than wavefronts)
+    const uint32_t s0 = KS ? wave * S / 4 : 0, some = KS ? (wave + 1) * S / 4 - s0 : S;
+    const uint32_t ns = some ? some : 1;
     const uint32_t first = KS ? blockIdx.x : blockIdx.x * 4 + wave;
     const uint32_t stride = KS ? gridDim.x : gridDim.x * 4;
     unsigned long long best = 0;
-    for (uint32_t gr = first; gr < ngroups; gr += stride) {
-        // row 16 gr + j: block 4 gr + j / 4 (clamped: rows past n are not used)
-        const uint32_t blk = min(4 * gr + (j >> 2), nblk - 1);
-        const int16_t* wp = w + ((size_t)blk * S * 4 + (j & 3)) * 128 + 8 * g;
-        v4u buf[2][4];
-        auto load = [&](int set, uint32_t s) {
+    // The table's pieces of AHEAD steps are in flight, across groups: what is
+    // past the last group repeats its rows.
+    v4u buf[AHEAD][4];
+    uint32_t lg = first, ls = 0;
+    const int16_t* lp;
+    auto group_rows = [&]() {
+        // row 16 lg + j: block 4 lg + j / 4 (clamped: rows past n are not used)
+        const uint32_t blk = min(4 * lg + (j >> 2), nblk - 1);
+        lp = w + (((size_t)blk * S + s0) * 4 + (j & 3)) * 128 + 8 * g;
+    };
+    group_rows();
+    const uint32_t rot = first % ns;
+    auto turn = [&](uint32_t s) { return s + rot < ns ? s + rot : s + rot - ns; };
+    auto load = [&](v4u* set) {
 #pragma unroll
-            for (int q = 0; q < 4; q++) buf[set][q] = *(const v4u*)(wp + (size_t)s * 512 + 32 * q);
-        };
-        v4i ha = {0, 0, 0, 0}, la = ha, sa = ha, sb = ha;  // a x, b x, a, b
-        auto step = [&](int set, uint32_t s) {
-#pragma unroll
-            for (int c = 0; c < 2; c++) {
-                const v4u u = buf[set][2 * c], v = buf[set][2 * c + 1];
-                const v4i a = {(int32_t)__builtin_amdgcn_perm(u.y, u.x, 0x07050301u),
-                               (int32_t)__builtin_amdgcn_perm(u.w, u.z, 0x07050301u),
-                               (int32_t)__builtin_amdgcn_perm(v.y, v.x, 0x07050301u),
-                               (int32_t)__builtin_amdgcn_perm(v.w, v.z, 0x07050301u)};
-                v4i b = {(int32_t)__builtin_amdgcn_perm(u.y, u.x, 0x06040200u),
-                         (int32_t)__builtin_amdgcn_perm(u.w, u.z, 0x06040200u),
-                         (int32_t)__builtin_amdgcn_perm(v.y, v.x, 0x06040200u),
-                         (int32_t)__builtin_amdgcn_perm(v.w, v.z, 0x06040200u)};
-                b ^= v4i{(int32_t)0x80808080u, (int32_t)0x80808080u, (int32_t)0x80808080u,
-                         (int32_t)0x80808080u};
-                const v4i xv = *(const v4i*)(lm_x + ((s * 2 + c) * 64 + lane) * 16);
-                ha = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, xv, ha, 0, 0, 0);
-                la = __builtin_amdgcn_mfma_i32_16x16x64_i8(b, xv, la, 0, 0, 0);
-                sa = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, ones, sa, 0, 0, 0);
-                sb = __builtin_amdgcn_mfma_i32_16x16x64_i8(b, ones, sb, 0, 0, 0);
-            }
-        };
-        if (s0 < s1) {
-            load(0, s0);
-            for (uint32_t s = s0; s < s1; s += 2) {
-                load(1, s + 1 < s1 ? s + 1 : s);
-                step(0, s);
-                load(0, s + 2 < s1 ? s + 2 : s);
-                if (s + 1 < s1) step(1, s + 1);
-            }
+        for (int q = 0; q < 4; q++) set[q] = *(const v4u*)(lp + (size_t)turn(ls) * 512 + 32 * q);
+        if (++ls == ns) {
+            ls = 0;
+            lg += stride;
+            group_rows();
         }
-        if constexpr (KS) {
-            red[wave][0][lane] = ha;
-            red[wave][1][lane] = la;
-            red[wave][2][lane] = sa;
-            red[wave][3][lane] = sb;
-            __syncthreads();
-            if (wave == 0) {
+    };
+    auto swap8 = [](int32_t v) {
+        return __builtin_amdgcn_update_dpp(0, v, 0x128, 0xf, 0xf, false);  // row_ror:8
+    };
+    v4i ha = {0, 0, 0, 0}, la = ha, sa = ha, sb = ha;  // a x, b x, a, b
+    auto step = [&](const v4u* set, uint32_t s) {
 #pragma unroll
-                for (int q = 1; q < 4; q++) {
-                    ha += red[q][0][lane];
-                    la += red[q][1][lane];
-                    sa += red[q][2][lane];
-                    sb += red[q][3][lane];
-                }
+        for (int c = 0; c < 2; c++) {
+            const v4u u = set[2 * c], v = set[2 * c + 1];
+            const v4i a = {(int32_t)__builtin_amdgcn_perm(u.y, u.x, 0x07050301u),
+                           (int32_t)__builtin_amdgcn_perm(u.w, u.z, 0x07050301u),
+                           (int32_t)__builtin_amdgcn_perm(v.y, v.x, 0x07050301u),
+                           (int32_t)__builtin_amdgcn_perm(v.w, v.z, 0x07050301u)};
+            v4i b = {(int32_t)__builtin_amdgcn_perm(u.y, u.x, 0x06040200u),
+                     (int32_t)__builtin_amdgcn_perm(u.w, u.z, 0x06040200u),
+                     (int32_t)__builtin_amdgcn_perm(v.y, v.x, 0x06040200u),
+                     (int32_t)__builtin_amdgcn_perm(v.w, v.z, 0x06040200u)};
+            b ^= v4i{(int32_t)0x80808080u, (int32_t)0x80808080u, (int32_t)0x80808080u,
+                     (int32_t)0x80808080u};
+            const v4i xv = *(const v4i*)(lm_x + ((s * 2 + c) * 64 + lane) * 16);
+            ha = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, xv, ha, 0, 0, 0);
+            la = __builtin_amdgcn_mfma_i32_16x16x64_i8(b, xv, la, 0, 0, 0);
+            sa = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, ones, sa, 0, 0, 0);
+            sb = __builtin_amdgcn_mfma_i32_16x16x64_i8(b, ones, sb, 0, 0, 0);
+        }
+    };
+    // the scores of group gr, the workgroup's it-th
+    auto finish = [&](uint32_t gr, uint32_t it) {
+        v4i sab = 256 * sa + sb;
+        if constexpr (KS) {
+            // one wavefront after the other adds the others' sums to its own;
+            // the next group's go to the other half
+            const uint32_t slot = (wave - it - 1) & 3;
+            if (!some) ha = la = sab = v4i{0, 0, 0, 0};
+            auto& rd = red[it & 1];
+            if (slot != 3) {
+                rd[slot][0][lane] = ha;
+                rd[slot][1][lane] = la;
+                rd[slot][2][lane] = sab;
             }
-            __syncthreads();
+            lds_barrier();
+            if (slot != 3) return;
+#pragma unroll
+            for (int q = 0; q < 3; q++) {
+                ha += rd[q][0][lane];
+                la += rd[q][1][lane];
+                sab += rd[q][2][lane];
+            }
         }
         // lane (j, g) holds table rows 16 gr + 4 g + t: column j < 8 the sums
-        // with row j's c, column j + 8 those with its d
+        // with row j's c, column j + 8 those with its d; it takes t = 0, 1 (j <
+        // 8) or 2, 3 of row j % 8, the other column's from lane j +- 8
+        const bool low = j < 8;
+        int64_t score[2];
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            const int32_t ad = __builtin_amdgcn_update_dpp(0, ha[t], 0x128, 0xf, 0xf, false);
-            const int32_t bd = __builtin_amdgcn_update_dpp(0, la[t], 0x128, 0xf, 0xf, false);
-            const int64_t score = 65536 * (int64_t)ha[t] + 256 * ((int64_t)ad + la[t]) + bd +
-                                  128 * (256 * (int64_t)sa[t] + sb[t] + xsum[j & 7]);
-            const uint32_t v = kLmGroup * gr + 4 * g + t;
-            const unsigned long long k = argmax_key(score, v);
+        for (int i = 0; i < 2; i++) {
+            const int32_t h = low ? ha[i] : ha[2 + i], l = low ? la[i] : la[2 + i];
+            // (what the other lane wants of this one)
+            const int32_t ho = swap8(low ? ha[2 + i] : ha[i]), lo = swap8(low ? la[2 + i] : la[i]);
+            score[i] = 65536 * (int64_t)(low ? h : ho) +
+                       256 * ((int64_t)(low ? ho : h) + (low ? l : lo)) + (low ? lo : l) +
+                       128 * ((int64_t)(low ? sab[i] : sab[2 + i]) + xsum[j & 7]);
+            const uint32_t v = kLmGroup * gr + 4 * g + (low ? 0 : 2) + i;
+            const unsigned long long k = argmax_key(score[i], v);
             if (v < n && k > best) best = k;
-            if (SC && j < rows && v < n && (!KS || wave == 0))
-                scores[(size_t)j * lds + v] = score;
+        }
+        // (the scores end with the last whole group)
+        if (SC && (j & 7) < rows)
+            *(v4u*)(scores + score_at(kLmGroup * gr + 4 * g + (low ? 0 : 2), j & 7, rows)) =
+                v4u{(uint32_t)score[0], (uint32_t)((uint64_t)score[0] >> 32), (uint32_t)score[1],
+                    (uint32_t)((uint64_t)score[1] >> 32)};
+    };
+    if (first < ngroups) {
+#pragma unroll
+        for (uint32_t i = 0; i < AHEAD; i++) load(buf[i]);
+        uint32_t gr = first, s = 0, it = 0;
+        for (bool more = true; more;) {
+#pragma unroll
+            for (uint32_t i = 0; i < AHEAD; i++) {
+                step(buf[i], s0 + turn(s));
+                load(buf[i]);
+                if (++s == ns) {
+                    finish(gr, it++);
+                    ha = la = sa = sb = v4i{0, 0, 0, 0};
+                    s = 0;
+                    gr += stride;
+                    more = gr < ngroups;
+                    if (!more) break;
+                }
+            }
         }
     }
-    // the best of a row's lanes (g), then of the wavefronts
+    // the best of a row's lanes, then of the wavefronts
 #pragma unroll
-    for (int o = 16; o < 64; o *= 2) {
+    for (int o = 8; o < 64; o *= 2) {
         const unsigned long long k = __shfl_xor(best, o);
         best = k > best ? k : best;
     }
@@ -1230,7 +1278,7 @@ __global__ __launch_bounds__(256) void lm_argmax_mfma_kernel(const int16_t* __re
     __syncthreads();
     if (tid < 8 && tid < rows) {
         unsigned long long k = 0;
-        for (int q = 0; q < (KS ? 1 : 4); q++) k = wbest[q][tid] > k ? wbest[q][tid] : k;
+        for (int q = 0; q < 4; q++) k = wbest[q][tid] > k ? wbest[q][tid] : k;
         atomicMax(&keys[tid], k);
     }
 }
@@ -1238,7 +1286,7 @@ __global__ __launch_bounds__(256) void lm_argmax_mfma_kernel(const int16_t* __re
 template <int RT, bool SC>
 static hipError_t launch_lm_rt(const int16_t* w, uint32_t steps, uint32_t n,
                                const int16_t* x, uint32_t ldx, uint32_t rows, int L,
-                               unsigned long long* keys, int64_t* scores, uint32_t lds,
+                               unsigned long long* keys, int64_t* scores,
                                hipStream_t st) {
     const uint32_t nblocks = (n + 3) / 4;
     // Every workgroup ends with one atomicMax per row on the same line, and
@@ -1257,20 +1305,20 @@ static hipError_t launch_lm_rt(const int16_t* w, uint32_t steps, uint32_t n,
     if (staged) {
         constexpr bool XS = RT <= 2;
         switch (L) {
-        case 0: lm_argmax_kernel<RT, 0, XS, SC><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys, scores, lds); break;
-        case 1: lm_argmax_kernel<RT, 1, XS, SC><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys, scores, lds); break;
-        case 4: lm_argmax_kernel<RT, 4, XS, SC><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys, scores, lds); break;
-        case 8: lm_argmax_kernel<RT, 8, XS, SC><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys, scores, lds); break;
-        default: lm_argmax_kernel<RT, 16, XS, SC><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys, scores, lds); break;
+        case 0: lm_argmax_kernel<RT, 0, XS, SC><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys, scores); break;
+        case 1: lm_argmax_kernel<RT, 1, XS, SC><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys, scores); break;
+        case 4: lm_argmax_kernel<RT, 4, XS, SC><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys, scores); break;
+        case 8: lm_argmax_kernel<RT, 8, XS, SC><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys, scores); break;
+        default: lm_argmax_kernel<RT, 16, XS, SC><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys, scores); break;
         }
         return hipGetLastError();
     }
     switch (L) {
-    case 0: lm_argmax_kernel<RT, 0, false, SC><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys, scores, lds); break;
-    case 1: lm_argmax_kernel<RT, 1, false, SC><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys, scores, lds); break;
-    case 4: lm_argmax_kernel<RT, 4, false, SC><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys, scores, lds); break;
-    case 8: lm_argmax_kernel<RT, 8, false, SC><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys, scores, lds); break;
-    default: lm_argmax_kernel<RT, 16, false, SC><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys, scores, lds); break;
+    case 0: lm_argmax_kernel<RT, 0, false, SC><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys, scores); break;
+    case 1: lm_argmax_kernel<RT, 1, false, SC><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys, scores); break;
+    case 4: lm_argmax_kernel<RT, 4, false, SC><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys, scores); break;
+    case 8: lm_argmax_kernel<RT, 8, false, SC><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys, scores); break;
+    default: lm_argmax_kernel<RT, 16, false, SC><<<grid, 256, 0, st>>>(w, steps, n, x, ldx, rows, keys, scores); break;
     }
     return hipGetLastError();
 }
@@ -1278,45 +1326,47 @@ static hipError_t launch_lm_rt(const int16_t* w, uint32_t steps, uint32_t n,
 template <bool SC>
 static hipError_t launch_lm(const int16_t* w, uint32_t steps, uint32_t n, const int16_t* x,
                             uint32_t ldx, uint32_t rows, int L, unsigned long long* keys,
-                            int64_t* scores, uint32_t lds, hipStream_t st) {
+                            int64_t* scores, hipStream_t st) {
     // From three rows on the matrix cores (call times, dot2 -> matrix cores:
     // 151,936 x 2,048, 3 rows 236 -> 127-135 us, 8 415 -> 128-135; 151,936 x
     // 896 98 -> 57, 157 -> 57; 16,384 x 896 35 -> 22, 39 -> 22; 8,192 x 256
     // 25 -> 18, 26 -> 18.  One and two rows stay on dot2: 106-109 and 118-120,
-    // 65 and 61, 17 and 18, 15 and 15).  Tables of fewer groups than 2,048
-    // wavefronts can walk share each among a workgroup's wavefronts, at most
-    // 512 of them (their final atomics share a line: 30,000 rows of 2,048 in
-    // 38 us, 49 with a workgroup per group); larger ones take one workgroup
-    // per compute unit (512 and 1,024 workgroups: 153 and 139 us, their last
-    // round nearly empty).
+    // 65 and 61, 17 and 18, 15 and 15).  At most one workgroup per compute unit
+    // (512: 151,936 x 2,048 103.2 us and 102.4, 32,011 x 896 18.5 and 17.3,
+    // 8,192 x 256 11.7 and 8.2).  Four steps ahead, two where a wavefront has
+    // 16 steps or fewer (4 and 2 steps ahead: 151,936 x 2,048 with scores 112.8
+    // and 117.4 us; 32,011 x 896 17.3 and 16.3, 8,192 x 256 8.2 and 7.3).
     const uint32_t groups = (n + kLmGroup - 1) / kLmGroup;
-    const bool shared = groups < 2048;
-    if (rows >= 3 && steps <= (shared ? kLmMfmaStepsShared : kLmMfmaSteps)) {
+    const bool shared = steps <= kLmMfmaStepsShared;
+    if (rows >= 3 && (shared || (steps <= kLmMfmaSteps && groups >= 2048))) {
         const uint32_t bytes = steps * 2048;  // of LDS
-        if (shared)
-            lm_argmax_mfma_kernel<true, SC><<<std::min(groups, 512u), 256, bytes, st>>>(
-                w, steps, n, x, ldx, rows, keys, scores, lds);
+        const uint32_t grid = std::min(groups, 256u);
+        if (!shared)
+            lm_argmax_mfma_kernel<false, SC, 2>
+                <<<grid, 256, bytes, st>>>(w, steps, n, x, ldx, rows, keys, scores);
+        else if ((groups + 255) / 256 * ((steps + 3) / 4) > 16)
+            lm_argmax_mfma_kernel<true, SC, 4>
+                <<<grid, 256, bytes, st>>>(w, steps, n, x, ldx, rows, keys, scores);
         else
-            lm_argmax_mfma_kernel<false, SC><<<256, 256, bytes, st>>>(w, steps, n, x, ldx, rows,
-                                                                      keys, scores, lds);
+            lm_argmax_mfma_kernel<true, SC, 2>
+                <<<grid, 256, bytes, st>>>(w, steps, n, x, ldx, rows, keys, scores);
         return hipGetLastError();
     }
-    if (rows <= 1) return launch_lm_rt<1, SC>(w, steps, n, x, ldx, rows, L, keys, scores, lds, st);
-    if (rows <= 2) return launch_lm_rt<2, SC>(w, steps, n, x, ldx, rows, L, keys, scores, lds, st);
-    if (rows <= 4) return launch_lm_rt<4, SC>(w, steps, n, x, ldx, rows, L, keys, scores, lds, st);
-    return launch_lm_rt<8, SC>(w, steps, n, x, ldx, rows, L, keys, scores, lds, st);
+    if (rows <= 1) return launch_lm_rt<1, SC>(w, steps, n, x, ldx, rows, L, keys, scores, st);
+    if (rows <= 2) return launch_lm_rt<2, SC>(w, steps, n, x, ldx, rows, L, keys, scores, st);
+    if (rows <= 4) return launch_lm_rt<4, SC>(w, steps, n, x, ldx, rows, L, keys, scores, st);
+    return launch_lm_rt<8, SC>(w, steps, n, x, ldx, rows, L, keys, scores, st);
 }
 
 hipError_t launch_lm_argmax(const int16_t* w, uint32_t steps, uint32_t n,
                             const int16_t* x, uint32_t ldx, uint32_t rows, int L,
                             unsigned long long* keys, hipStream_t st) {
-    return launch_lm<false>(w, steps, n, x, ldx, rows, L, keys, nullptr, 0, st);
+    return launch_lm<false>(w, steps, n, x, ldx, rows, L, keys, nullptr, st);
 }
 hipError_t launch_lm_scores(const int16_t* w, uint32_t steps, uint32_t n,
                             const int16_t* x, uint32_t ldx, uint32_t rows, int L,
-                            unsigned long long* keys, int64_t* scores, uint32_t lds,
-                            hipStream_t st) {
-    return launch_lm<true>(w, steps, n, x, ldx, rows, L, keys, scores, lds, st);
+                            unsigned long long* keys, int64_t* scores, hipStream_t st) {
+    return launch_lm<true>(w, steps, n, x, ldx, rows, L, keys, scores, st);
 }
 
 // ---------------------------------------------------------------------

@@ -263,7 +263,7 @@ struct llm_ctx {
     // verification's words in pinned host memory.
     struct Probs {
         int64_t* scores = nullptr;
-        size_t lds = 0;
+        size_t tokens = 0;
         uint32_t* exp2 = nullptr;
         llm::DrawPlace* place = nullptr;
         unsigned long long *part = nullptr, *left = nullptr;
@@ -2930,12 +2930,12 @@ int ensure_probs(llm_ctx* c) {
     if (!b.host &&
         hipHostMalloc((void**)&b.host, 24 * sizeof(uint32_t), hipHostMallocDefault) != hipSuccess)
         return fail(LLM_E_NOMEM, "hipHostMalloc failed");
-    const size_t lds = round_up(c->lm_vocab, 16);
-    if (b.lds < lds) {
+    const size_t tokens = round_up(c->lm_vocab, 16);
+    if (b.tokens < tokens) {
         int64_t* p = nullptr;
-        if ((rc = dev_alloc(c, (void**)&p, 8 * lds * 8))) return rc;
+        if ((rc = dev_alloc(c, (void**)&p, 8 * tokens * 8))) return rc;
         b.scores = p;
-        b.lds = lds;
+        b.tokens = tokens;
     }
     return 0;
 }
@@ -2959,7 +2959,6 @@ int check_lm_rows(llm_ctx* c, uint32_t pair, uint32_t row0, uint32_t rows, const
 int enqueue_scores(llm_ctx* c, uint32_t pair, uint32_t row0, uint32_t rows, llm::ProbArgs& a) {
     llm_ctx::Probs& b = c->probs;
     a.scores = b.scores;
-    a.lds = (uint32_t)b.lds;
     a.vocab = c->lm_vocab;
     a.rows = rows;
     a.exp2 = b.exp2;
@@ -2970,7 +2969,7 @@ int enqueue_scores(llm_ctx* c, uint32_t pair, uint32_t row0, uint32_t rows, llm:
     c->busy = llm_ctx::WORK;
     HIP_TRY(llm::launch_lm_scores(c->lm.d, c->lm.steps, c->lm_vocab,
                                   c->pairs[pair] + (size_t)row0 * c->Hp, c->Hp, rows, c->lm.L,
-                                  c->lm_keys, b.scores, (uint32_t)b.lds, c->stream));
+                                  c->lm_keys, b.scores, c->stream));
     return 0;
 }
 

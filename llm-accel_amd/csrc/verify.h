@@ -25,8 +25,8 @@ struct DrawPlace {
 };
 
 struct ProbArgs {
-    const int64_t* scores;  // [rows][lds], 20 fraction bits
-    uint32_t lds, vocab, rows;
+    const int64_t* scores;  // score_at(token, row, rows), 20 fraction bits
+    uint32_t vocab, rows;
     const uint32_t* exp2;   // [2][kExp2Entries]: 2^-(i / 2^10), 2^-(i / 2^20) in 2^-30
     uint32_t inverse[8];    // per row log2(e) / temperature in 2^-24
     unsigned long long* keys;  // the rows' argmax keys; 0 once the call's work is done

@@ -114,13 +114,12 @@ __global__ __launch_bounds__(256) void prob_sums_kernel(ProbArgs a) {
     __shared__ uint32_t pdraft[8], taken[8], lds_last;
     const uint32_t tid = threadIdx.x, r = blockIdx.y, v0 = blockIdx.x * kSumChunk;
     const uint32_t chunks = gridDim.x, j = a.request[r], first = a.first[j], count = a.count[j];
-    const int64_t* s = a.scores + (size_t)r * a.lds;
     constexpr uint32_t kEach = kSumChunk / 256;
     int64_t sv[kEach];
 #pragma unroll
     for (uint32_t i = 0; i < kEach; i++) {
         const uint32_t v = v0 + 256 * i + tid;
-        sv[i] = s[v < a.vocab ? v : 0];
+        sv[i] = a.scores[score_at(v < a.vocab ? v : 0, r, a.rows)];
     }
     exp2_load(a.exp2, e);
     const int64_t top = (int64_t)(a.keys[r] >> 18) - ((int64_t)1 << 45);
@@ -149,7 +148,7 @@ __global__ __launch_bounds__(256) void prob_sums_kernel(ProbArgs a) {
     if (tid < count) {
         const uint32_t row = first + tid, x = a.draft[row];
         const uint64_t z = total[tid];
-        const int64_t below = row_top(tid) - a.scores[(size_t)row * a.lds + x];
+        const int64_t below = row_top(tid) - a.scores[score_at(x, row, a.rows)];
         const uint32_t p = prob32(weight(e, below, a.inverse[row]), z, 1.0 / (double)z);
         pdraft[tid] = p;
         taken[tid] = (uint64_t)a.accept_u[row] * drafted(a, j, tid, x) < (uint64_t)p << 32;
@@ -170,12 +169,11 @@ __global__ __launch_bounds__(256) void prob_sums_kernel(ProbArgs a) {
 __global__ __launch_bounds__(256) void probs_kernel(ProbArgs a, uint32_t* probs) {
     __shared__ __attribute__((aligned(16))) Exp2 e;
     const uint32_t tid = threadIdx.x, r = blockIdx.y, v0 = blockIdx.x * kProbChunk;
-    const int64_t* s = a.scores + (size_t)r * a.lds;
     int64_t sv[kProbChunk / 256];
 #pragma unroll
     for (uint32_t i = 0; i < kProbChunk / 256; i++) {
         const uint32_t v = v0 + 256 * i + tid;
-        sv[i] = s[v < a.vocab ? v : 0];
+        sv[i] = a.scores[score_at(v < a.vocab ? v : 0, r, a.rows)];
     }
     exp2_load(a.exp2, e);
     const uint64_t z = a.place[r].total;
@@ -205,7 +203,6 @@ __global__ __launch_bounds__(256) void draw_kernel(ProbArgs a) {
     const uint64_t z = a.place[j].total;
     const int64_t top = a.place[j].top;
     const double inv = 1.0 / (double)z;
-    const int64_t* s = a.scores + (size_t)row * a.lds;
     const uint32_t c = a.inverse[row];
     constexpr uint32_t kEach = kProbChunk / 256;
     // P of the thread's tokens of a chunk, and what of it lies above Q (`at`
@@ -218,7 +215,7 @@ __global__ __launch_bounds__(256) void draw_kernel(ProbArgs a) {
 #pragma unroll
         for (uint32_t i = 0; i < kEach; i++) {
             const uint32_t t = v + i;
-            sv[i] = s[t < a.vocab ? t : 0];
+            sv[i] = a.scores[score_at(t < a.vocab ? t : 0, row, a.rows)];
             q[i] = at < count && t < a.vocab ? drafted(a, j, at, t) : 0;
         }
         __syncthreads();  // (the tables, the first time)
