@@ -26,6 +26,7 @@
 // drawing its token.
 #include "verify.h"
 
+#include "attn_common.h"
 #include "coherent.h"
 #include "kernels.h"
 
@@ -67,31 +68,49 @@ __device__ __forceinline__ uint32_t prob32(uint32_t w, uint64_t z, double inv) {
     return q > 0xffffffffu ? 0xffffffffu : (uint32_t)q;
 }
 
-__device__ __forceinline__ unsigned long long wave_sum64(unsigned long long v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
+// Sum over the wavefront's lanes up to this one: within rows of 16 lanes, then
+// the row before's and the first half's (row_bcast).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned long long scan_step64(unsigned long long v) {
+    const uint32_t lo = (uint32_t)dpp<CTRL, ROWS>(0, (int32_t)v);
+    const uint32_t hi = (uint32_t)dpp<CTRL, ROWS>(0, (int32_t)(v >> 32));
+    return v + ((unsigned long long)hi << 32 | lo);
 }
-// Sum over the workgroup's 256 threads, uniform; red: 4 words.
-__device__ __forceinline__ unsigned long long block_sum64(unsigned long long v,
-                                                          unsigned long long* red) {
+__device__ __forceinline__ unsigned long long wave_scan64(unsigned long long v) {
+    v = scan_step64<0x111, 0xf>(v);  // row_shr:1, 2, 4, 8
+    v = scan_step64<0x112, 0xf>(v);
+    v = scan_step64<0x114, 0xf>(v);
+    v = scan_step64<0x118, 0xf>(v);
+    v = scan_step64<0x142, 0xa>(v);  // row_bcast:15, 31
+    return scan_step64<0x143, 0xc>(v);
+}
+// Over all of them, uniform.
+__device__ __forceinline__ unsigned long long wave_sum64(unsigned long long v) {
+    v = wave_scan64(v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int32_t)v, 63);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int32_t)(v >> 32), 63);
+    return (unsigned long long)hi << 32 | lo;
+}
+// Sums over the workgroup's 256 threads, uniform; red: 8 words.
+__device__ __forceinline__ void block_sums64(unsigned long long& u, unsigned long long& v,
+                                             unsigned long long* red) {
+    u = wave_sum64(u);
     v = wave_sum64(v);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 0) {
+        red[threadIdx.x >> 6] = u;
+        red[4 + (threadIdx.x >> 6)] = v;
+    }
     __syncthreads();
-    return red[0] + red[1] + red[2] + red[3];
+    u = red[0] + red[1] + red[2] + red[3];
+    v = red[4] + red[5] + red[6] + red[7];
 }
 
 // Sum of v over the threads below this one; red: 4 words.
 __device__ __forceinline__ unsigned long long block_below64(unsigned long long v,
                                                             unsigned long long* red) {
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    unsigned long long s = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const unsigned long long u = __shfl_up(s, o, 64);
-        if ((int)lane >= o) s += u;
-    }
+    unsigned long long s = wave_scan64(v);
     __syncthreads();
     if (lane == 63) red[wave] = s;
     __syncthreads();
@@ -129,7 +148,10 @@ __global__ __launch_bounds__(256) void prob_sums_kernel(ProbArgs a) {
 #pragma unroll
     for (uint32_t i = 0; i < kEach; i++)
         if (v0 + 256 * i + tid < a.vocab) sum += weight(e, top - sv[i], c);
-    sum = block_sum64(sum, red);
+    sum = wave_sum64(sum);
+    if ((tid & 63) == 0) red[tid >> 6] = sum;
+    __syncthreads();
+    sum = red[0] + red[1] + red[2] + red[3];
     if (tid == 0) st_coherent(&a.part[r * kSumChunksMax + blockIdx.x], sum);
     if (!arrive_last(a.count_in + 32 * r, chunks, &lds_last)) return;
     if (count && !arrive_last(a.count_in + 32 * (8 + j), count + 1, &lds_last)) return;
@@ -195,7 +217,7 @@ __global__ __launch_bounds__(256) void probs_kernel(ProbArgs a, uint32_t* probs)
 // request's next token is drawn from; its last workgroup draws it.
 __global__ __launch_bounds__(256) void draw_kernel(ProbArgs a) {
     __shared__ __attribute__((aligned(16))) Exp2 e;
-    __shared__ unsigned long long red[4], before;
+    __shared__ unsigned long long red[8], before;
     __shared__ uint32_t lds_last, chunk;
     const uint32_t tid = threadIdx.x, chunks = gridDim.x;
     const uint32_t j = blockIdx.y, first = a.first[j], count = a.count[j];
@@ -231,8 +253,7 @@ __global__ __launch_bounds__(256) void draw_kernel(ProbArgs a) {
     unsigned long long sl = 0, sp = 0;
 #pragma unroll
     for (uint32_t i = 0; i < kEach; i++) sl += above[i], sp += p[i];
-    sl = block_sum64(sl, red);
-    sp = block_sum64(sp, red);
+    block_sums64(sl, sp, red);
     if (chunks > 1) {
         unsigned long long* left = a.left + (size_t)j * kProbChunksMax * 2;
         if (tid == 0) {
@@ -248,7 +269,8 @@ __global__ __launch_bounds__(256) void draw_kernel(ProbArgs a) {
     } else if (tid != 0) {
         sl = sp = 0;
     }
-    const unsigned long long all_l = block_sum64(sl, red), all_p = block_sum64(sp, red);
+    unsigned long long all_l = sl, all_p = sp;
+    block_sums64(all_l, all_p, red);
     const bool whole = all_l == 0;  // nothing above Q: P itself
     const uint64_t sum = whole ? all_p : all_l;  // 1 .. 2^32
     const uint64_t t = ((uint64_t)a.sample_u[j] * sum) >> 32;
