@@ -13,9 +13,11 @@
 // The weights of the shared projection bound a call and are read once for
 // all rows, by the projection's own kernels, which leave their exact sums in
 // `wide`, while other workgroups of the same launch form x A^T; A and B of an
-// adapter are read once for all rows under it.  Both
-// are the caller's row-major memory (adapters come and go with requests), B
-// as [rank][outputs] so that a wavefront reads consecutive outputs.
+// adapter are read once for all rows under it.  Both are the caller's row-major
+// memory (adapters come and go with requests), B as [rank][outputs] so that a
+// wavefront reads consecutive outputs.  Launch boundaries are what a small call
+// waits for: one row of 2,048 x 2,048 took 17.8 us in four launches (a copy of
+// the row, the projection, x A^T, this one) and takes 10 in these two.
 #include "adapter.h"
 
 #include "proj_common.h"
@@ -25,7 +27,9 @@ namespace {
 
 // Workgroup (128 outputs, group): wavefront w takes every fourth rank from w
 // on, a lane two outputs, sixteen ranks' loads at a time; the wavefronts' sums
-// meet in LDS.
+// meet in LDS.  Bound by two dependent loads (t, then what B's loads left) and
+// the sums' exchange: 3.8 us for one row of rank 16, 4.6 for 8 rows under
+// adapters of their own of rank 64 (2.1 MB of B), 2,048 outputs each.
 constexpr uint32_t kOutCols = 128, kAhead = 16;
 __global__ __launch_bounds__(256) void adapter_out_kernel(AdapterArgs a) {
     __shared__ int64_t red[4][8][kOutCols];

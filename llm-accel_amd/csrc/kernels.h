@@ -12,7 +12,7 @@ namespace llm {
 // optionally write a constant-gain RMSNorm of the result); SILU store
 // silu(gate) * up; STORE_NORM_IN like STORE on inputs normalised while they
 // are loaded (constant-gain RMSNorm of the raw rows); WIDE stores the exact
-// sums themselves (ProjArgs::wide).
+// sums themselves (64 bits each).
 enum { EPI_STORE = 0, EPI_RESID = 1, EPI_SILU = 2, EPI_STORE_NORM_IN = 3, EPI_WIDE = 4 };
 
 // Rows per weight block and columns per k-step of the "tile4x128" layout.
@@ -26,7 +26,7 @@ struct ProjArgs {
     uint32_t steps;     // K_pad / 128
     const int16_t* x;   // activations [rows][ldx], ldx >= K_pad
     uint32_t ldx;
-    int16_t* out;       // [rows][ldo]
+    int16_t* out;       // [rows][ldo] (EPI_WIDE: int64 sums, 20 fraction bits)
     uint32_t ldo;
     const int16_t* res; // residual [rows][ldr] (EPI_RESID)
     uint32_t ldr;
@@ -77,7 +77,6 @@ struct ProjArgs {
     // copy holds the clamped value; unused words are 0.
     const uint32_t* corr0;
     const uint32_t* corr1;
-    int64_t* wide;  // EPI_WIDE: the sums [rows][ldo], 20 fraction bits
 };
 // EPI_WIDE: rows past `rows` are not read (x may be a caller's memory), and
 // the workgroups past the projection's own `blocks` form x A^T of the rows'

@@ -1920,7 +1920,8 @@ int enqueue_op_projection(llm_ctx* c, uint32_t layer, uint32_t proj, uint32_t T,
     ad->x = in;
     ad->inputs = m.k;
     ad->outputs = n;
-    ad->wide = a.wide = c->op_wide;
+    ad->wide = c->op_wide;
+    a.out = (int16_t*)c->op_wide;
     ad->t = c->op_t;
     ad->out = out;
     a.ad = *ad;
