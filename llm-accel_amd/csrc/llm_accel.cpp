@@ -1894,7 +1894,7 @@ int enqueue_op_projection(llm_ctx* c, uint32_t layer, uint32_t proj, uint32_t T,
     else
         HIP_TRY(hipMemcpy2DAsync(c->op_stage, (size_t)m.k_pad * 2, in, (size_t)m.k * 2,
                                  (size_t)m.k * 2, T, hipMemcpyDeviceToDevice, c->stream));
-    llm::ProjWideArgs a{};
+    llm::ProjArgs a{};
     a.w0 = m.d ? m.d + (size_t)row0 * m.k_pad : nullptr;
     a.steps = m.steps;
     a.x = direct ? in : c->op_stage;
@@ -1921,11 +1921,11 @@ int enqueue_op_projection(llm_ctx* c, uint32_t layer, uint32_t proj, uint32_t T,
     ad->inputs = m.k;
     ad->outputs = n;
     ad->wide = c->op_wide;
-    a.out = (int16_t*)c->op_wide;
     ad->t = c->op_t;
     ad->out = out;
-    a.ad = *ad;
-    HIP_TRY(llm::launch_proj(a, llm::EPI_WIDE, m.L, (uint32_t)cdiv(n, 4), c->stream));
+    a.out = (int16_t*)c->op_wide;
+    const llm::ProjWideArgs aw{a, *ad, 0};
+    HIP_TRY(llm::launch_proj(aw, llm::EPI_WIDE, m.L, (uint32_t)cdiv(n, 4), c->stream));
     HIP_TRY(llm::launch_adapter_out(*ad, c->stream));
     return 0;
 }

@@ -266,3 +266,13 @@ def test_refuses_more_tiles_than_a_launch_counts():
         acc.attention_shared(0, 0, 63, out, p, p, p, 1 << 14, out)
         acc.sync()
         assert not hip.get(out, 63 * 16 * 16, np.int16).any()
+
+
+@pytest.mark.gpu
+def test_nothing_to_attend_to():
+    """No prefix and no own rows at all: zeros, and nothing behind them."""
+    with _accelerator(6, 3, 48, 64) as acc, Hip() as hip:
+        rng = np.random.default_rng(3)
+        q = _full(rng, 5, 6, 48)
+        none = np.zeros((5, 3, 0, 48), np.int16)
+        assert not _call(acc, hip, 0, q, none, none, [0] * 5).any()
