@@ -364,3 +364,25 @@ def test_refusals_of_a_context():
                 acc.lm_head_verify(*args)
         with pytest.raises(llm_accel.AccelError):
             acc.lm_head_verify(0, 0, [1], [1], [0], [0], [1.0], out + 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hidden,heads,vocab,rows", [
+    (2048, 16, 40001, 8), (2048, 16, 40001, 3), (2816, 22, 9000, 5), (2944, 23, 32770, 8),
+    (3840, 30, 33003, 3), (3968, 31, 2050, 8)])
+def test_probabilities_of_wide_heads(hidden, heads, vocab, rows):
+    """Every way that the scores are computed in: groups shared with four steps
+    ahead, a group per wavefront, and no matrix cores."""
+    rng = np.random.default_rng([9, hidden, vocab, rows])
+    table, x = _table(rng, vocab, hidden), _rows(rng, rows, hidden)
+    table[vocab // 3], x[rows - 1] = -32768, -32768
+    temperatures = [float(t) for t in rng.choice([0.7, 20.0, 64.0], rows)]
+    with llm_accel.Accelerator(llm_accel.Shape(vocab, hidden, 128, 1, heads, heads, 64,
+                                               1e6)) as acc, Hip() as hip:
+        acc.load_lm_head(table)
+        got = _device_probs(acc, hip, x, temperatures, vocab)
+        scores = _scores(x, table)
+        for r in range(rows):
+            assert np.array_equal(got[r], _probs_row(scores[r], temperatures[r])), r
+        toks, best = acc.lm_head_argmax(0, 0, rows)
+        assert toks == scores.argmax(1).tolist() and best == scores.max(1).tolist()

@@ -276,3 +276,34 @@ def test_nothing_to_attend_to():
         q = _full(rng, 5, 6, 48)
         none = np.zeros((5, 3, 0, 48), np.int16)
         assert not _call(acc, hip, 0, q, none, none, [0] * 5).any()
+
+
+@pytest.mark.gpu
+def test_two_contexts_and_calls_of_changing_sizes():
+    """Calls of two contexts in turn, none waited for, larger and smaller ones
+    over the same scratch: each finds its own."""
+    rng = np.random.default_rng(21)
+    heads, kv, d, cached = 14, 2, 64, 1400
+    sizes = [(1400, 9, 200), (130, 3, 5), (700, 20, 90), (0, 2, 700), (1400, 1, 0), (64, 33, 257)]
+    with _accelerator(heads, kv, d, cached) as a0, _accelerator(heads, kv, d, cached) as a1, \
+            Hip() as hip:
+        accs, caches, calls = (a0, a1), [], []
+        for acc in accs:
+            k, v = _normal(rng, 1.5, kv, cached, d), _normal(rng, 0.5, kv, cached, d)
+            _fill(acc, 0, k, v)
+            caches.append((k, v))
+        for prefix, seqs, cap in sizes:
+            for i in (0, 1):
+                q, ko, vo = (_normal(rng, s, *sh) for s, sh in (
+                    (2.0, (seqs, heads, d)), (1.5, (seqs, kv, cap, d)), (0.5, (seqs, kv, cap, d))))
+                lengths = rng.integers(0, cap + 1, seqs).astype(np.uint32)
+                calls.append((i, prefix, q, ko, vo, lengths, hip.put(q), hip.put(ko), hip.put(vo),
+                              hip.put(lengths), hip.alloc(q.nbytes)))
+        for _ in range(2):
+            for i, prefix, q, ko, vo, lengths, dq, dk, dv, dl, out in calls:
+                accs[i].attention_shared(0, prefix, len(q), dq, dk, dv, dl, ko.shape[2], out)
+        a0.sync(), a1.sync()
+        for i, prefix, q, ko, vo, lengths, *_, out in calls:
+            want = _expected(q, *caches[i], ko, vo, lengths, prefix)
+            got = hip.get(out, q.shape, np.int16)
+            assert np.array_equal(got, want), (i, prefix, first_mismatch(got, want))
