@@ -18,8 +18,8 @@
 //   join     per (row, head elements): the chain over the tiles.
 // Measured back to back, 16 query heads in 2 KV groups of 128: 8 sequences,
 // 16,000 + up to 300 positions (17.7 MB of K and V, 2.9 us at 6.2 TB/s) 7.0, 9.1
-// and 7.7 us, together 25.5; 32 sequences, 8,100 + up to 600: 12.2, 17.7 and
-// 12.2, together 42.5.  The first are dependent steps (loads, conversion,
+// and 7.7 us, together 25.5; 32 sequences, 8,100 + up to 600: 12.2, 16.7 and
+// 9.9, together 39.1.  The first are dependent steps (loads, conversion,
 // products, exchange, store) and launch boundaries, not bytes; the second work:
 // 1,648 tiles' jobs of 64 rows, and 36 MB of tile values written and read.
 // A prefix tile is one job for all sequences (16 query rows per product: the
@@ -491,8 +491,13 @@ struct ValueSmem {
     int16_t hist[4][kJobRows];   // per wavefront, running maximum of its tiles
     uint32_t far;                // a V value saturates
     uint32_t pad[3];
-    int8_t planes[kJobPieces][4][1024];  // p, c(p); own tiles use the first
-    int16_t vt[128 * kOwnRow];   // own tiles
+    union {
+        int8_t planes[kJobPieces][4][1024];  // p, c(p) of the pieces
+        struct {                             // own tiles have one
+            int8_t planes[4][1024];
+            int16_t vt[128 * kOwnRow];
+        } own;
+    };
 };
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 
@@ -506,6 +511,7 @@ __device__ __forceinline__ void value_job(const SharedAttnArgs& a, const Job& b,
     const uint32_t d = a.head_dim, ne = d / 16, nrows = b.end - b.rho;
     // this tile's rows from b.rho on
     const size_t trow = ((size_t)b.h * a.tiles + b.j) * a.rows_pad + b.rho;
+    auto planes_of = [&](uint32_t piece) { return OWN ? sm.own.planes : sm.planes[piece]; };
     v4u raw[ES][2];
     if (!OWN) {
         const int16_t* page = a.vcache + ((size_t)b.h * a.pages + b.j) * TILE * d;
@@ -539,7 +545,7 @@ __device__ __forceinline__ void value_job(const SharedAttnArgs& a, const Job& b,
         for (uint32_t t = tid >> 3; t < b.j; t += 32)
             m = __builtin_elementwise_max(m, *(const s16x8*)(tm + (size_t)t * a.rows_pad));
     }
-    if (OWN) own_values(a, b, sm.vt);
+    if (OWN) own_values(a, b, sm.own.vt);
     *(v4u*)(sm.e14 + 8 * tid) = table;
     if (tid == 0) {
         *(v4u*)(sm.e14 + 2048) = last;
@@ -570,7 +576,7 @@ __device__ __forceinline__ void value_job(const SharedAttnArgs& a, const Job& b,
         const int32_t top = max(before, tmj);
         const int32_t sum = quad_sum(row_probs<OWN>(
             s0, s1, top, (int32_t)b.valid - 16 * (int32_t)g, sm.e14, pw));
-        prob_planes(pw, lane, sm.planes[w]);
+        prob_planes(pw, lane, planes_of(w));
         if (g == 0 && 16 * w + q < nrows) {
             a.tsum[trow + r] = sum << 2;
             a.old[trow + r] = (int32_t)sm.e14[max(before - top, -2048) + 2048] << 2;
@@ -582,7 +588,7 @@ __device__ __forceinline__ void value_job(const SharedAttnArgs& a, const Job& b,
     for (int es = 0; es < ES; es++) {
         if (OWN) {
             const uint32_t e = 16 * min(w + 4 * es, ne - 1) + q;
-            const int16_t* p = sm.vt + e * kOwnRow + 16 * g;
+            const int16_t* p = sm.own.vt + e * kOwnRow + 16 * g;
             planes16(*(const v4u*)p, *(const v4u*)(p + 8), va[es], vb[es], even, odd);
         } else {
             planes16(unpair8(raw[es][0]), unpair8(raw[es][1]), va[es], vb[es], even, odd);
@@ -592,7 +598,7 @@ __device__ __forceinline__ void value_job(const SharedAttnArgs& a, const Job& b,
     __syncthreads();
     const bool vf = sm.far != 0;
     if (vf) {
-        if (piece) prob_corr(pw, lane, sm.planes[w]);
+        if (piece) prob_corr(pw, lane, planes_of(w));
         __syncthreads();
     }
     // ---- values ----
@@ -602,7 +608,7 @@ __device__ __forceinline__ void value_job(const SharedAttnArgs& a, const Job& b,
         const bool real = r0 + q < nrows;
 #pragma unroll
         for (int es = 0; es < ES; es++) {
-            const v2u tv = strip_values(va[es], vb[es], vf, lane, sm.planes[r0 / 16]);
+            const v2u tv = strip_values(va[es], vb[es], vf, lane, planes_of(r0 / 16));
             const uint32_t st = w + 4 * es;
             if (real && st < ne) *(v2u*)(out + (r0 + q) * d + 16 * st) = tv;
         }
@@ -628,8 +634,10 @@ __global__ __launch_bounds__(256, 4) void shared_values_kernel(SharedAttnArgs a)
 // are past) is one addition of its sum, four such runs at a time: exact,
 // because the probabilities' sums are not negative and the elements' 32 values
 // (at most 2^28 together) cannot saturate an accumulator within 2^30.
+// RUNS: of a block, by as many groups of 8 threads.
+template <uint32_t RUNS>
 __global__ __launch_bounds__(256) void shared_join_kernel(SharedAttnArgs a) {
-    constexpr uint32_t EC = 8, RUNS = 256 / EC, BLOCK = 8 * RUNS;
+    constexpr uint32_t EC = 8, BLOCK = 8 * RUNS;
     __shared__ __attribute__((aligned(16))) int16_t s_v[BLOCK][8 * EC];
     __shared__ __attribute__((aligned(16))) int32_t s_run[RUNS][8 * EC];
     __shared__ __attribute__((aligned(16))) int32_t s_old[BLOCK], s_sum[BLOCK];
@@ -640,7 +648,7 @@ __global__ __launch_bounds__(256) void shared_join_kernel(SharedAttnArgs a) {
     const uint32_t seq = __umul24(rho, a.inv_group) >> 16;
     const size_t at = (size_t)h * a.tiles * a.rows_pad + rho;
     const uint32_t step = a.rows_pad;
-    const bool real = 8 * ec < ne;
+    const bool mine = run < RUNS, real = mine && 8 * ec < ne;
     v4u v[8];
     int32_t old = 65536, ts = 0;
     // (bounded by the tiles there can be: nothing waits for the length)
@@ -668,15 +676,17 @@ __global__ __launch_bounds__(256) void shared_join_kernel(SharedAttnArgs a) {
         for (uint32_t u = 0; u < 8; u++) {
             // tiles that this sequence does not have hold anything
             if (first + u >= nt) v[u] = v4u{0, 0, 0, 0};
-            *(v4u*)&s_v[8 * run + u][8 * ec] = v[u];
+            if (mine) *(v4u*)&s_v[8 * run + u][8 * ec] = v[u];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 lo[i] = dot2(v[u][i], 0x00000001u, lo[i]);
                 hi[i] = dot2(v[u][i], 0x00010000u, hi[i]);
             }
         }
-        *(v4i*)&s_run[run][8 * ec] = v4i{lo[0], hi[0], lo[1], hi[1]};
-        *(v4i*)&s_run[run][8 * ec + 4] = v4i{lo[2], hi[2], lo[3], hi[3]};
+        if (mine) {
+            *(v4i*)&s_run[run][8 * ec] = v4i{lo[0], hi[0], lo[1], hi[1]};
+            *(v4i*)&s_run[run][8 * ec + 4] = v4i{lo[2], hi[2], lo[3], hi[3]};
+        }
         if (tid < BLOCK) {
             const bool there = t0 + tid < nt;
             int32_t o = there ? old : 65536, z = there ? ts : 0;
@@ -947,7 +957,14 @@ hipError_t launch_shared_attention(const SharedAttnArgs& a, hipStream_t st) {
     e = hipGetLastError();
     if (e != hipSuccess) return e;
     const dim3 rows(a.kv_heads * a.rows, (a.head_dim + 63) / 64);
-    shared_join_kernel<<<rows, 256, 0, st>>>(a);
+    // 32 runs take 43 KB of LDS (3 workgroups per compute unit), 28 take 38 (4):
+    // the larger blocks where all rows' workgroups run at once all the same (255
+    // tiles: 7.7 us and 8.9), the smaller where they do not (1,024 workgroups,
+    // 136 tiles: 12.2 and 9.9)
+    if (rows.x * rows.y > 3 * 256)
+        shared_join_kernel<28><<<rows, 256, 0, st>>>(a);
+    else
+        shared_join_kernel<32><<<rows, 256, 0, st>>>(a);
     return hipGetLastError();
 }
 
