@@ -268,7 +268,7 @@ struct llm_ctx {
         llm::DrawPlace* place = nullptr;
         unsigned long long *part = nullptr, *left = nullptr;
         uint32_t* count = nullptr;
-        uint32_t* host = nullptr;
+        unsigned long long* host = nullptr;
     } probs;
 
     // Request loop (llm_generate): pinned staging of the embedding rows of
@@ -2927,10 +2927,13 @@ int ensure_probs(llm_ctx* c) {
     if (!b.place && (rc = dev_alloc(c, (void**)&b.place, 8 * sizeof(llm::DrawPlace)))) return rc;
     if (!b.part && (rc = dev_alloc(c, (void**)&b.part, 8 * llm::kSumChunksMax * 8))) return rc;
     if (!b.left && (rc = dev_alloc(c, (void**)&b.left, 8 * llm::kProbChunksMax * 16))) return rc;
-    if (!b.count && (rc = dev_alloc(c, (void**)&b.count, 17 * 32 * 4))) return rc;
-    if (!b.host &&
-        hipHostMalloc((void**)&b.host, 24 * sizeof(uint32_t), hipHostMallocDefault) != hipSuccess)
-        return fail(LLM_E_NOMEM, "hipHostMalloc failed");
+    if (!b.count && (rc = dev_alloc(c, (void**)&b.count, 16 * 32 * 4))) return rc;
+    if (!b.host) {
+        if (hipHostMalloc((void**)&b.host, 24 * sizeof(*b.host), hipHostMallocDefault) !=
+            hipSuccess)
+            return fail(LLM_E_NOMEM, "hipHostMalloc failed");
+        std::memset(b.host, 0, 24 * sizeof(*b.host));
+    }
     const size_t tokens = round_up(c->lm_vocab, 16);
     if (b.tokens < tokens) {
         int64_t* p = nullptr;
@@ -3042,16 +3045,31 @@ int llm_lm_head_verify(llm_ctx_t* c, uint32_t pair, uint32_t row0, uint32_t requ
     a.q = nd ? draft_probs : nullptr;
     a.left = c->probs.left;
     a.host = c->probs.host;
-    a.flag = c->io_flag;
     a.seq = ++c->io_seq;
     HIP_TRY(llm::launch_verify(a, c->stream));
-    if (int rc = io_wait(c, a.seq)) return rc;
-    if (int rc = check_waits(c)) return rc;
-    for (uint32_t j = 0; j < requests; j++) {
-        accepted[j] = a.host[j];
-        tokens[j] = a.host[8 + j];
+    // as io_wait(), every word carrying the call's number
+    uint32_t words[24];
+    auto arrived = [&](uint32_t at, uint32_t n) {
+        for (uint32_t i = at; i < at + n; i++) {
+            const unsigned long long w = __atomic_load_n(a.host + i, __ATOMIC_ACQUIRE);
+            if ((uint32_t)(w >> 32) != a.seq) return false;
+            words[i] = (uint32_t)w;
+        }
+        return true;
+    };
+    auto all = [&] { return arrived(0, requests) && arrived(8, requests) && arrived(16, rows); };
+    bool done = false;
+    for (uint32_t i = 0; i < 200000 && !(done = all()); i++) __builtin_ia32_pause();
+    if (!done) {
+        HIP_TRY(hipStreamSynchronize(c->stream));
+        if (!all()) return fail(LLM_E_HIP, "a verification's result did not arrive");
     }
-    if (probs) std::memcpy(probs, a.host + 16, rows * sizeof(uint32_t));
+    c->busy = llm_ctx::QUIET;
+    c->copies_open = false;
+    if (int rc = check_waits(c)) return rc;
+    std::copy(words, words + requests, accepted);
+    std::copy(words + 8, words + 8 + requests, tokens);
+    if (probs) std::copy(words + 16, words + 16 + rows, probs);
     return 0;
 }
 

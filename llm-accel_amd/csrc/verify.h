@@ -40,15 +40,14 @@ struct ProbArgs {
     // per row and chunk the sum of its weights, per request what comes of them
     unsigned long long* part;  // [8][kSumChunksMax]
     DrawPlace* place;          // [8]
-    uint32_t* count_in;        // [17 * 32] arrivals, a line per row, per request and
-                               // of all requests (zero between launches)
+    uint32_t* count_in;        // [16 * 32] arrivals, a line per row and per request
+                               // (zero between launches)
     // per request and chunk the sums of what a token is drawn from (the part
     // above q, and p itself)
     unsigned long long* left;  // [8][kProbChunksMax][2]
-    // pinned host memory: accepted[8], token[8], prob[8 rows], and the word
-    // that receives seq once they are visible
-    uint32_t* host;
-    uint32_t* flag;
+    // pinned host memory: accepted[8], token[8], prob[8 rows], each with seq in
+    // its upper half (no word waits for another)
+    unsigned long long* host;
     uint32_t seq;
 };
 // Q0.32 probabilities probs[r][v], tight rows: every row a request without
