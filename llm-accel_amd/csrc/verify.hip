@@ -129,12 +129,114 @@ __device__ __forceinline__ uint32_t drafted(const ProbArgs& a, uint32_t j, uint3
     return v == a.draft[a.first[j] + i] ? 0xffffffffu : 0u;
 }
 
+// The chunk's part of the distribution that request j's next token is drawn
+// from (row `at` of it, whose weights' sum and largest score are z and top);
+// the request's last workgroup of `chunks` draws it.  The tables are in e.
+struct DrawSmem {
+    unsigned long long red[8], before;
+    uint32_t last, chunk;
+};
+__device__ __forceinline__ void draw_chunk(const ProbArgs& a, const Exp2& e, DrawSmem& sm,
+                                           uint32_t own, uint32_t chunks, uint32_t j, uint32_t at,
+                                           uint64_t z, int64_t top, const uint32_t* pdraft) {
+    const uint32_t tid = threadIdx.x, first = a.first[j], count = a.count[j], row = first + at;
+    const double inv = 1.0 / (double)z;
+    const uint32_t c = a.inverse[row];
+    constexpr uint32_t kEach = kProbChunk / 256;
+    // P of the thread's tokens of a chunk, and what of it lies above Q (`at`
+    // past the drafts: all of it)
+    uint32_t p[kEach], above[kEach];
+    auto fill = [&](uint32_t ch) {
+        const uint32_t v = ch * kProbChunk + kEach * tid;
+        int64_t sv[kEach];
+        uint32_t q[kEach];
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; i++) {
+            const uint32_t t = v + i;
+            sv[i] = a.scores[score_at(t < a.vocab ? t : 0, row, a.rows)];
+            q[i] = at < count && t < a.vocab ? drafted(a, j, at, t) : 0;
+        }
+        __syncthreads();  // (the tables, the first time)
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; i++) {
+            p[i] = 0;
+            if (v + i < a.vocab) p[i] = prob32(weight(e, top - sv[i], c), z, inv);
+            above[i] = p[i] > q[i] ? p[i] - q[i] : 0;
+        }
+    };
+    fill(own);
+    unsigned long long sl = 0, sp = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; i++) sl += above[i], sp += p[i];
+    block_sums64(sl, sp, sm.red);
+    if (chunks > 1) {
+        unsigned long long* left = a.left + (size_t)j * kProbChunksMax * 2;
+        if (tid == 0) {
+            st_coherent(&left[2 * own], sl);
+            st_coherent(&left[2 * own + 1], sp);
+        }
+        if (!arrive_last(a.count_in + 32 * j, chunks, &sm.last)) return;
+        sl = sp = 0;
+        if (tid < chunks) {
+            sl = ld_coherent(&left[2 * tid]);
+            sp = ld_coherent(&left[2 * tid + 1]);
+        }
+    } else if (tid != 0) {
+        sl = sp = 0;
+    }
+    unsigned long long all_l = sl, all_p = sp;
+    block_sums64(all_l, all_p, sm.red);
+    const bool whole = all_l == 0;  // nothing above Q: P itself
+    const uint64_t sum = whole ? all_p : all_l;  // 1 .. 2^32
+    const uint64_t t = ((uint64_t)a.sample_u[j] * sum) >> 32;
+    // the chunk, then the thread's tokens of it, whose running sum passes t:
+    // one thread of the workgroup each time
+    const unsigned long long mass_c = whole ? sp : sl;
+    const unsigned long long below_c = block_below64(mass_c, sm.red);
+    if (t >= below_c && t < below_c + mass_c) {
+        sm.chunk = tid;
+        sm.before = below_c;
+    }
+    __syncthreads();
+    const uint32_t ch = sm.chunk;
+    if (ch != own) fill(ch);
+    unsigned long long mine = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; i++) {
+        if (whole) above[i] = p[i];
+        mine += above[i];
+    }
+    auto tell = [&](uint32_t i, uint32_t v) {
+        __hip_atomic_store(a.host + i, (unsigned long long)a.seq << 32 | v, __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_SYSTEM);
+    };
+    uint64_t lower = sm.before + block_below64(mine, sm.red);
+    if (t >= lower && t < lower + mine) {
+        uint32_t at_i = 0, pv = p[0];
+#pragma unroll
+        for (uint32_t i = 0; i + 1 < kEach; i++)
+            if (at_i == i && lower + above[i] <= t) {
+                lower += above[i];
+                at_i = i + 1;
+                pv = p[i + 1];
+            }
+        tell(j, at);
+        tell(8 + j, ch * kProbChunk + kEach * tid + at_i);
+        tell(16 + first + count, pv);
+    }
+    if (tid < count) tell(16 + first + tid, pdraft[tid]);
+    if (tid <= count) a.keys[first + tid] = 0;  // nothing of this launch reads them
+}
+
 // Workgroup (chunk, row): the sum of the chunk's weights.  The last one of a
-// request tests its drafts.
+// request tests its drafts and, where a chunk of draws holds the vocabulary
+// (DRAW), draws its token too.
+template <bool DRAW>
 __global__ __launch_bounds__(256) void prob_sums_kernel(ProbArgs a) {
     __shared__ __attribute__((aligned(16))) Exp2 e;
-    __shared__ unsigned long long red[4], total[8];
-    __shared__ uint32_t pdraft[8], taken[8], lds_last;
+    __shared__ DrawSmem sm;
+    __shared__ unsigned long long total[8];
+    __shared__ uint32_t pdraft[8], taken[8], place;
     const uint32_t tid = threadIdx.x, r = blockIdx.y, v0 = blockIdx.x * kSumChunk;
     const uint32_t chunks = gridDim.x, j = a.request[r], first = a.first[j], count = a.count[j];
     constexpr uint32_t kEach = kSumChunk / 256;
@@ -153,16 +255,16 @@ __global__ __launch_bounds__(256) void prob_sums_kernel(ProbArgs a) {
     for (uint32_t i = 0; i < kEach; i++)
         if (v0 + 256 * i + tid < a.vocab) sum += weight(e, top - sv[i], c);
     sum = wave_sum64(sum);
-    if ((tid & 63) == 0) red[tid >> 6] = sum;
+    if ((tid & 63) == 0) sm.red[tid >> 6] = sum;
     __syncthreads();
-    sum = red[0] + red[1] + red[2] + red[3];
+    sum = sm.red[0] + sm.red[1] + sm.red[2] + sm.red[3];
     if (tid == 0) st_coherent(&a.part[r * kSumChunksMax + blockIdx.x], sum);
     // few arrivals on one line (15 ns each), else a row's first (~1 us more)
     if (chunks * (count + 1) <= 64) {
-        if (!arrive_last(a.count_in + 32 * (8 + j), chunks * (count + 1), &lds_last)) return;
+        if (!arrive_last(a.count_in + 32 * (8 + j), chunks * (count + 1), &sm.last)) return;
     } else {
-        if (!arrive_last(a.count_in + 32 * r, chunks, &lds_last)) return;
-        if (count && !arrive_last(a.count_in + 32 * (8 + j), count + 1, &lds_last)) return;
+        if (!arrive_last(a.count_in + 32 * r, chunks, &sm.last)) return;
+        if (count && !arrive_last(a.count_in + 32 * (8 + j), count + 1, &sm.last)) return;
     }
 
     // the rows' sums, a wavefront at a time
@@ -188,12 +290,21 @@ __global__ __launch_bounds__(256) void prob_sums_kernel(ProbArgs a) {
     if (tid == 0) {
         uint32_t at = 0;
         while (at < count && taken[at]) at++;
-        DrawPlace* o = &a.place[j];
-        o->total = total[at];
-        o->top = row_top(at);
-        o->at = at;
+        place = at;
+        if (!DRAW) {
+            DrawPlace* o = &a.place[j];
+            o->total = total[at];
+            o->top = row_top(at);
+            o->at = at;
+        }
     }
-    if (tid < count) a.place[j].pdraft[tid] = pdraft[tid];
+    if constexpr (DRAW) {
+        __syncthreads();
+        const uint32_t at = place;
+        draw_chunk(a, e, sm, 0, 1, j, at, total[at], row_top(at), pdraft);
+    } else {
+        if (tid < count) a.place[j].pdraft[tid] = pdraft[tid];
+    }
 }
 
 // Workgroup (chunk, row): the chunk's probabilities.
@@ -222,104 +333,12 @@ __global__ __launch_bounds__(256) void probs_kernel(ProbArgs a, uint32_t* probs)
     if (blockIdx.x == 0 && r == 0 && tid < 8) a.keys[tid] = 0;
 }
 
-// Workgroup (chunk, request): the chunk's part of the distribution that the
-// request's next token is drawn from; its last workgroup draws it.
 __global__ __launch_bounds__(256) void draw_kernel(ProbArgs a) {
     __shared__ __attribute__((aligned(16))) Exp2 e;
-    __shared__ unsigned long long red[8], before;
-    __shared__ uint32_t lds_last, chunk;
-    const uint32_t tid = threadIdx.x, chunks = gridDim.x;
-    const uint32_t j = blockIdx.y, first = a.first[j], count = a.count[j];
-    const uint32_t at = a.place[j].at, row = first + at;
-    const uint64_t z = a.place[j].total;
-    const int64_t top = a.place[j].top;
-    const double inv = 1.0 / (double)z;
-    const uint32_t c = a.inverse[row];
-    constexpr uint32_t kEach = kProbChunk / 256;
-    // P of the thread's tokens of a chunk, and what of it lies above Q (`at`
-    // past the drafts: all of it)
-    uint32_t p[kEach], above[kEach];
-    auto fill = [&](uint32_t ch) {
-        const uint32_t v = ch * kProbChunk + kEach * tid;
-        int64_t sv[kEach];
-        uint32_t q[kEach];
-#pragma unroll
-        for (uint32_t i = 0; i < kEach; i++) {
-            const uint32_t t = v + i;
-            sv[i] = a.scores[score_at(t < a.vocab ? t : 0, row, a.rows)];
-            q[i] = at < count && t < a.vocab ? drafted(a, j, at, t) : 0;
-        }
-        __syncthreads();  // (the tables, the first time)
-#pragma unroll
-        for (uint32_t i = 0; i < kEach; i++) {
-            p[i] = 0;
-            if (v + i < a.vocab) p[i] = prob32(weight(e, top - sv[i], c), z, inv);
-            above[i] = p[i] > q[i] ? p[i] - q[i] : 0;
-        }
-    };
+    __shared__ DrawSmem sm;
     exp2_load(a.exp2, e);
-    fill(blockIdx.x);
-    unsigned long long sl = 0, sp = 0;
-#pragma unroll
-    for (uint32_t i = 0; i < kEach; i++) sl += above[i], sp += p[i];
-    block_sums64(sl, sp, red);
-    if (chunks > 1) {
-        unsigned long long* left = a.left + (size_t)j * kProbChunksMax * 2;
-        if (tid == 0) {
-            st_coherent(&left[2 * blockIdx.x], sl);
-            st_coherent(&left[2 * blockIdx.x + 1], sp);
-        }
-        if (!arrive_last(a.count_in + 32 * j, chunks, &lds_last)) return;
-        sl = sp = 0;
-        if (tid < chunks) {
-            sl = ld_coherent(&left[2 * tid]);
-            sp = ld_coherent(&left[2 * tid + 1]);
-        }
-    } else if (tid != 0) {
-        sl = sp = 0;
-    }
-    unsigned long long all_l = sl, all_p = sp;
-    block_sums64(all_l, all_p, red);
-    const bool whole = all_l == 0;  // nothing above Q: P itself
-    const uint64_t sum = whole ? all_p : all_l;  // 1 .. 2^32
-    const uint64_t t = ((uint64_t)a.sample_u[j] * sum) >> 32;
-    // the chunk, then the thread's tokens of it, whose running sum passes t:
-    // one thread of the workgroup each time
-    const unsigned long long mass_c = whole ? sp : sl;
-    const unsigned long long below_c = block_below64(mass_c, red);
-    if (t >= below_c && t < below_c + mass_c) {
-        chunk = tid;
-        before = below_c;
-    }
-    __syncthreads();
-    const uint32_t ch = chunk;
-    if (ch != blockIdx.x) fill(ch);
-    unsigned long long mine = 0;
-#pragma unroll
-    for (uint32_t i = 0; i < kEach; i++) {
-        if (whole) above[i] = p[i];
-        mine += above[i];
-    }
-    auto tell = [&](uint32_t i, uint32_t v) {
-        __hip_atomic_store(a.host + i, (unsigned long long)a.seq << 32 | v, __ATOMIC_RELAXED,
-                           __HIP_MEMORY_SCOPE_SYSTEM);
-    };
-    uint64_t lower = before + block_below64(mine, red);
-    if (t >= lower && t < lower + mine) {
-        uint32_t at_i = 0, pv = p[0];
-#pragma unroll
-        for (uint32_t i = 0; i + 1 < kEach; i++)
-            if (at_i == i && lower + above[i] <= t) {
-                lower += above[i];
-                at_i = i + 1;
-                pv = p[i + 1];
-            }
-        tell(j, at);
-        tell(8 + j, ch * kProbChunk + kEach * tid + at_i);
-        tell(16 + first + count, pv);
-    }
-    if (tid < count) tell(16 + first + tid, a.place[j].pdraft[tid]);
-    if (tid <= count) a.keys[first + tid] = 0;  // nothing of this launch reads them
+    const DrawPlace& o = a.place[blockIdx.y];
+    draw_chunk(a, e, sm, blockIdx.x, gridDim.x, blockIdx.y, o.at, o.total, o.top, o.pdraft);
 }
 
 uint32_t chunks_of(const ProbArgs& a, uint32_t each) { return (a.vocab + each - 1) / each; }
@@ -327,7 +346,7 @@ uint32_t chunks_of(const ProbArgs& a, uint32_t each) { return (a.vocab + each - 
 }  // namespace
 
 hipError_t launch_probs(const ProbArgs& a, uint32_t* probs, hipStream_t st) {
-    prob_sums_kernel<<<dim3(chunks_of(a, kSumChunk), a.rows), 256, 0, st>>>(a);
+    prob_sums_kernel<false><<<dim3(chunks_of(a, kSumChunk), a.rows), 256, 0, st>>>(a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     probs_kernel<<<dim3(chunks_of(a, kProbChunk), a.rows), 256, 0, st>>>(a, probs);
@@ -335,7 +354,11 @@ hipError_t launch_probs(const ProbArgs& a, uint32_t* probs, hipStream_t st) {
 }
 
 hipError_t launch_verify(const ProbArgs& a, hipStream_t st) {
-    prob_sums_kernel<<<dim3(chunks_of(a, kSumChunk), a.rows), 256, 0, st>>>(a);
+    if (a.vocab <= kProbChunk) {
+        prob_sums_kernel<true><<<dim3(1, a.rows), 256, 0, st>>>(a);
+        return hipGetLastError();
+    }
+    prob_sums_kernel<false><<<dim3(chunks_of(a, kSumChunk), a.rows), 256, 0, st>>>(a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     draw_kernel<<<dim3(chunks_of(a, kProbChunk), a.requests), 256, 0, st>>>(a);
