@@ -26,8 +26,8 @@
 // probabilities, or the draws, a request's last workgroup drawing its token.
 // Dependent round trips bound those (arrivals, the chunks' sums, the chunk
 // again, the words to the host, ~1 us each), not the scores' bytes: sums of 8
-// rows 10.3 us at 151,936 tokens, 8.0 at 32,011, 6.8 at 1,024; draws 12.1, 12.1
-// and 7.4; probabilities of 8 rows 4.7 at 32,011.
+// rows 10.3 us at 151,936 tokens, 7.5 at 32,011; draws 11.4 and 11.1; both in
+// one launch, 4 rows of 1,024, 11.0; probabilities of 8 rows 4.7 at 32,011.
 #include "verify.h"
 
 #include "attn_common.h"
@@ -354,6 +354,8 @@ hipError_t launch_probs(const ProbArgs& a, uint32_t* probs, hipStream_t st) {
 }
 
 hipError_t launch_verify(const ProbArgs& a, hipStream_t st) {
+    // a vocabulary of one chunk: 1,024 tokens 24.1 us a call, 26.3 with the draws
+    // in a launch of their own, which larger ones need for their chunks
     if (a.vocab <= kProbChunk) {
         prob_sums_kernel<true><<<dim3(1, a.rows), 256, 0, st>>>(a);
         return hipGetLastError();
