@@ -172,8 +172,7 @@ template <int EPI, bool COH = false>
 __device__ __forceinline__ void proj_out(const ProjArgs& a, uint32_t r, uint32_t n,
                                          int64_t t0, int64_t t1, const EpiIn& ei) {
     if (EPI == EPI_WIDE) {
-        // (out's type serves: a member more in every launch's arguments cost a
-        // decode forward 0.5 us a layer)
+        // (out serves, so that the other launches' arguments stay as they are)
         ((int64_t*)a.out)[(size_t)r * a.ldo + n] = t0;
         return;
     }
